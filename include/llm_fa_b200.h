@@ -184,6 +184,132 @@ int llmfa_forward_static_scratch(const void* q, const int64_t q_strides[3], cons
  */
 int llmfa_selftest_wait_timeout(uint32_t timeout_us, void* stream);
 
+/* ---------------------------------------------------------------- 4-bit key/value cache
+ *
+ * A paged cache that holds keys and values in 4 bits, attention over it, and
+ * eviction from it by the attention weight that its tokens received. Head dim
+ * 128; no counterpart in the reference. All calls are stream-ordered, allocate
+ * nothing and can be captured in a CUDA graph (after one eager call of any
+ * entry point on the device).
+ *
+ * Device data is not readable before the launch, so what it may hold wrong is
+ * found by the kernels and reported in the device status word
+ * (llmfa_device_status): a page id outside the pool or a token without a page
+ * (the token is not written, counts as absent, or reads as zeros), a length or
+ * count outside its range (clamped), a move from outside the sequence (not
+ * made).
+ */
+#define LLMFA_DEVICE_STATUS_KV4_BAD_PAGE 0x2001
+#define LLMFA_DEVICE_STATUS_KV4_BAD_LENGTH 0x2002
+#define LLMFA_DEVICE_STATUS_KV4_BAD_SOURCE 0x2003
+
+/* Types of queries, keys, values and outputs. */
+#define LLMFA_BF16 0
+#define LLMFA_FP16 1
+
+/* The pool. A page holds page_size (16, 32, 64, 128 or 256) tokens of every
+ * key/value head: pages[num_pages][heads][llmfa_kv4_page_bytes()], 16-byte
+ * aligned, laid out in blocks of 16 tokens (16 x 64 bytes of key codes, 16 x
+ * 128/group (scale, zero) pairs of bf16, then the same of values). group (32,
+ * 64 or 128) channels share a pair: a code u stands for scale * (u - zero).
+ * positions and weights are [num_pages][heads][page_size]: the position that a
+ * token was appended at and the attention weight that it has accumulated. */
+typedef struct llmfa_kv4_cache {
+  void* pages;
+  int32_t* positions;
+  float* weights;
+  int64_t num_pages;
+  int32_t heads;
+  int32_t page_size;
+  int32_t group;
+} llmfa_kv4_cache;
+
+/* The sequences of a call (at most 4096): slot i of sequence b is in page
+ * page_table[b * table_stride + i / page_size]. lengths[b] slots hold tokens.
+ * No two sequences may share a page that a call writes. */
+typedef struct llmfa_kv4_seqs {
+  const int32_t* page_table;
+  int64_t table_stride;
+  int64_t max_pages;
+  const int32_t* lengths;
+  int64_t batch;
+} llmfa_kv4_seqs;
+
+/* Bytes of one page of one head. */
+int llmfa_kv4_page_bytes(int32_t page_size, int32_t group, uint64_t* bytes);
+
+/*
+ * Quantises k, v [batch, tokens, heads, 128] (strides of batch, token, head as
+ * for llmfa_forward) into slots lengths[b] .. lengths[b] + counts[b] - 1 of
+ * each sequence. counts = NULL: all `tokens`; rows past a count are not read.
+ * A token's position is seen[b] + its index (seen = NULL: lengths[b]), its
+ * weight 0. lengths is not changed: the layers of a model share it.
+ * Over a group of channels with lo = min(0, x), hi = max(0, x): scale =
+ * bf16((hi - lo) / 15), zero = round(-lo / scale), code = clamp(round(x /
+ * scale) + zero, 0, 15). Groups with an infinity or NaN read back as NaN; a
+ * scale below 2^-120 counts as 0.
+ */
+int llmfa_kv4_append(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, const void* k,
+                     const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
+                     const int32_t* counts, const int32_t* seen, int64_t tokens, int dtype,
+                     void* stream);
+
+/*
+ * Reads slots lengths[b] .. lengths[b] + counts[b] - 1 back into k, v [batch,
+ * tokens, heads, 128]; rows past a count are zeros. (seqs->lengths is the
+ * first slot to read here.)
+ */
+int llmfa_kv4_expand(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, void* k,
+                     const int64_t k_strides[3], void* v, const int64_t v_strides[3],
+                     const int32_t* counts, int64_t tokens, int dtype, void* stream);
+
+/* Workspace of llmfa_kv4_attention, 16-byte aligned. Its contents are not read
+ * across calls; calls that share one must not overlap. */
+int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t heads_q,
+                                       int64_t tokens, uint64_t* bytes);
+
+/*
+ * o = softmax(q k^T * softmax_scale) v for the last counts[b] tokens of each
+ * sequence (counts = NULL: all `tokens`); q, o are [batch, tokens, heads_q,
+ * 128], heads_q a multiple of the cache's heads, query head i reading key head
+ * i / (heads_q / heads). seqs->lengths counts the new tokens, whose keys are
+ * appended already. With causal != 0, new token i sees slots 0 .. lengths[b] -
+ * counts[b] + i, else all. A row that sees no slot gets zeros (and lse -inf);
+ * rows past a count are left as they were. lse as for llmfa_forward_lse, or
+ * NULL. decay >= 0 (at most 1) tracks: weights[slot] = decay * weights[slot] +
+ * the slot's softmax weights summed over the new tokens and the query heads of
+ * its head; with decay 0 the old value is not read. decay < 0 leaves weights
+ * alone.
+ */
+int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, const void* q,
+                        const int64_t q_strides[3], void* o, const int64_t o_strides[3],
+                        float* lse, const int64_t lse_strides[2], const int32_t* counts,
+                        int64_t heads_q, int64_t tokens, int causal, float softmax_scale,
+                        float decay, int dtype, void* workspace, uint64_t workspace_bytes,
+                        void* stream);
+
+/* Workspace of llmfa_kv4_evict_select, 16-byte aligned. */
+int llmfa_kv4_evict_workspace_size(int64_t batch, int64_t heads, int64_t keep, uint64_t* bytes);
+
+/*
+ * Chooses what leaves when sequence b is cut to keep slots: of every head the
+ * lengths[b] - keep tokens of least weight, the lowest slot first among equals
+ * (NaN counts as the largest weight); tokens at the `recent` (at most keep)
+ * latest positions, seen[b] - recent and on (seen = NULL: lengths[b] -
+ * recent), go after all others. The freed slots below keep take, in ascending
+ * order, the surviving tokens at or above it: src[b][head][d] is the slot
+ * whose token slot d is to hold, -1 past the new length min(lengths[b], keep),
+ * which new_lengths[b] receives (it must not be seqs->lengths itself).
+ */
+int llmfa_kv4_evict_select(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs,
+                           const int32_t* seen, int64_t keep, int64_t recent, int32_t* src,
+                           int32_t* new_lengths, void* workspace, uint64_t workspace_bytes,
+                           void* stream);
+
+/* Makes the moves of src [batch][heads][keep] (seqs->lengths is not read). */
+int llmfa_kv4_evict_move(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs,
+                         const int32_t* src, int64_t keep, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,11 +21,35 @@ LLMFA_ERR_LAUNCH = 4
 LLMFA_ERR_CUDA = 5
 LLMFA_ERR_DEVICE_TIMEOUT = 6
 DEVICE_STATUS_TIMEOUT_BASE = 0x1000
+DEVICE_STATUS_KV4_BAD_PAGE = 0x2001
+DEVICE_STATUS_KV4_BAD_LENGTH = 0x2002
+DEVICE_STATUS_KV4_BAD_SOURCE = 0x2003
+LLMFA_BF16 = 0
+LLMFA_FP16 = 1
 
 _I64x3 = ctypes.c_int64 * 3
 _I64x2 = ctypes.c_int64 * 2
 _lock = threading.Lock()
 _lib = None
+
+
+
+class Kv4Cache(ctypes.Structure):
+    """llmfa_kv4_cache."""
+    _fields_ = [("pages", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("weights", ctypes.c_void_p), ("num_pages", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("group", ctypes.c_int32)]
+
+
+class Kv4Seqs(ctypes.Structure):
+    """llmfa_kv4_seqs."""
+    _fields_ = [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("max_pages", ctypes.c_int64), ("lengths", ctypes.c_void_p),
+                ("batch", ctypes.c_int64)]
+
+
+_KV4 = [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Seqs)]
 
 # name -> (restype, argtypes); every function declared in include/llm_fa_b200.h
 SIGNATURES = {
@@ -62,6 +86,29 @@ SIGNATURES = {
     "llmfa_selftest_wait_timeout": (ctypes.c_int, [ctypes.c_uint32, ctypes.c_void_p]),
     "llmfa_trace_read": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint64,
                                         ctypes.POINTER(ctypes.c_uint64)]),
+    "llmfa_kv4_page_bytes": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32,
+                                            ctypes.POINTER(ctypes.c_uint64)]),
+    "llmfa_kv4_append": (ctypes.c_int, _KV4 + [
+        ctypes.c_void_p, _I64x3, ctypes.c_void_p, _I64x3, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_int64, ctypes.c_int, ctypes.c_void_p]),
+    "llmfa_kv4_expand": (ctypes.c_int, _KV4 + [
+        ctypes.c_void_p, _I64x3, ctypes.c_void_p, _I64x3, ctypes.c_void_p, ctypes.c_int64,
+        ctypes.c_int, ctypes.c_void_p]),
+    "llmfa_kv4_attention_workspace_size": (ctypes.c_int, [
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+        ctypes.POINTER(ctypes.c_uint64)]),
+    "llmfa_kv4_attention": (ctypes.c_int, _KV4 + [
+        ctypes.c_void_p, _I64x3, ctypes.c_void_p, _I64x3, ctypes.c_void_p,
+        ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_uint64, ctypes.c_void_p]),
+    "llmfa_kv4_evict_workspace_size": (ctypes.c_int, [
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_uint64)]),
+    "llmfa_kv4_evict_select": (ctypes.c_int, _KV4 + [
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]),
+    "llmfa_kv4_evict_move": (ctypes.c_int, _KV4 + [ctypes.c_void_p, ctypes.c_int64,
+                                                   ctypes.c_void_p]),
 }
 
 

@@ -27,8 +27,9 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB = PKG / "libllm_fa_b200.so"
-SOURCES = [CSRC / "llm_fa_api.cu"]
-DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
+SOURCES = [CSRC / "llm_fa_api.cu", CSRC / "kv4_api.cu"]
+DEPS = (SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
+        + sorted(INCLUDE.glob("*.h")))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

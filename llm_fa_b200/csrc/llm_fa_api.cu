@@ -21,6 +21,7 @@
 
 #include "../../include/llm_fa_b200.h"
 #include "fa_fwd_kernel.cuh"
+#include "setup.h"
 
 namespace {
 
@@ -196,6 +197,14 @@ __global__ void llmfa_wait_selftest_kernel(unsigned long long timeout_ns, int* s
 }
 
 }  // namespace
+
+int llmfa::device_status_ptr(int** out) {
+  int dev = 0;
+  DeviceSetup* s = nullptr;
+  const int rc = device_setup(&dev, &s);
+  if (rc == LLMFA_OK) *out = s->status_ptr;
+  return rc;
+}
 
 extern "C" {
 
