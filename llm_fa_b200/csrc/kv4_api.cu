@@ -3,8 +3,10 @@
 // synchronisation; every check is made before the first CUDA call.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/llm_fa_b200.h"
 #include "kv4_attention.cuh"
@@ -84,6 +86,129 @@ int64_t quant_blocks(int64_t rows) {
   return (rows * kKv4RowThreads + kKv4QuantThreads - 1) / kKv4QuantThreads;
 }
 
+// Rows of a key head, cut into tiles of 8 nt: the least padding of 8, 16 or 32.
+struct AttnShape {
+  int64_t batch, heads, heads_q, tokens;
+  int nt, row_tiles;
+  int64_t units;
+};
+
+int attn_shape(int64_t batch, int64_t heads, int64_t heads_q, int64_t tokens, AttnShape* s) {
+  if (batch < 1 || heads < 1 || heads_q < 1 || tokens < 1 || heads_q % heads != 0)
+    return LLMFA_ERR_INVALID_ARGUMENT;
+  if (batch > kKv4MaxBatch || heads_q >= (1 << 24) || tokens >= (1 << 24) ||
+      batch * heads_q >= (int64_t(1) << 31) / tokens)
+    return LLMFA_ERR_UNSUPPORTED;
+  const int64_t rows = tokens * (heads_q / heads);
+  const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  const int64_t tiles = (rows + 8 * nt - 1) / (8 * nt);
+  *s = AttnShape{batch, heads, heads_q, tokens, nt, static_cast<int>(tiles), batch * heads * tiles};
+  return LLMFA_OK;
+}
+
+// CTAs of the attention kernel per SM and their shape.
+template <int NT>
+struct AttnConfig;
+template <>
+struct AttnConfig<1> {
+  static constexpr int kWarps = 8, kStages = 2, kCtas = 2;
+};
+template <>
+struct AttnConfig<2> {
+  static constexpr int kWarps = 12, kStages = 2, kCtas = 1;
+};
+template <>
+struct AttnConfig<4> {
+  static constexpr int kWarps = 8, kStages = 3, kCtas = 1;
+};
+
+int attn_ctas(int nt, int sms) {
+  return sms * (nt == 1 ? AttnConfig<1>::kCtas : nt == 2 ? AttnConfig<2>::kCtas : AttnConfig<4>::kCtas);
+}
+
+struct AttnLayout {  // byte offsets in the workspace; partial outputs come first
+  uint64_t ml, unit, row_lse, bytes;
+};
+
+// The grid uses at most this many SMs (a B200 has 148), so that the workspace's size follows from
+// a call's arguments alone.
+constexpr int kMaxSms = 160;
+
+AttnLayout attn_layout(const AttnShape& s) {
+  const uint64_t rows = uint64_t(2) * attn_ctas(s.nt, kMaxSms) * 8 * s.nt;
+  AttnLayout w;
+  w.ml = rows * kKv4Dim * sizeof(float);
+  w.unit = w.ml + rows * sizeof(float2);
+  w.row_lse = w.unit + static_cast<uint64_t>(s.units) * sizeof(int2);
+  w.bytes = w.row_lse + static_cast<uint64_t>(s.batch * s.heads_q * s.tokens) * sizeof(float);
+  return w;
+}
+
+// A launch that may start while the kernel before it ends, and waits for it itself.
+template <typename K>
+int launch_after(K kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t st,
+                 const Kv4AttnParams& p) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+    cudaGetLastError();
+    return LLMFA_ERR_LAUNCH;
+  }
+  return LLMFA_OK;
+}
+
+// The kernel may use `bytes` of shared memory; asked for once a device.
+template <auto Kernel>
+int allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return LLMFA_ERR_CUDA;
+  }
+  if (((done.load(std::memory_order_acquire) >> dev) & 1) != 0) return LLMFA_OK;
+  if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(bytes)) != cudaSuccess) {
+    cudaGetLastError();
+    return LLMFA_ERR_CUDA;
+  }
+  done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  return LLMFA_OK;
+}
+
+template <typename T, int NT, int NG>
+int attn_launch(Kv4AttnParams& p, const AttnShape& shape, int sms, cudaStream_t st) {
+  using C = AttnConfig<NT>;
+  constexpr auto kernel = kv4_attention_kernel<T, NT, NG, C::kWarps, C::kStages, C::kCtas>;
+  using Smem = Kv4AttnSmem<NT, NG, C::kWarps, C::kStages>;
+  constexpr size_t kMost = sizeof(Smem) + (kKv4MaxBatch + 1) * sizeof(uint32_t);
+  static_assert(kMost <= 227 * 1024, "shared memory");
+  const size_t prefix = static_cast<size_t>(shape.batch + 1) * sizeof(uint32_t);
+  int rc;
+  if ((rc = allow_smem<kernel>(kMost)) != LLMFA_OK) return rc;
+  p.ctas = sms * C::kCtas;
+  kernel<<<static_cast<unsigned>(p.ctas), C::kWarps * 32, sizeof(Smem) + prefix, st>>>(p);
+  if ((rc = launched()) != LLMFA_OK) return rc;
+  if ((rc = launch_after(kv4_combine_kernel<T, NT>, static_cast<unsigned>(shape.units),
+                         kKv4CombineThreads, 0, st, p)) != LLMFA_OK)
+    return rc;
+  if (p.row_lse == nullptr) return LLMFA_OK;
+  constexpr auto weights = kv4_weights_kernel<T, NT, NG, 8, 3, 2>;
+  using WSmem = Kv4WeightsSmem<NT, NG, 8, 3>;
+  constexpr size_t kMostW = sizeof(WSmem) + (kKv4MaxBatch + 1) * sizeof(uint32_t);
+  static_assert(2 * (kMostW + 1024) <= 228 * 1024, "shared memory");
+  if ((rc = allow_smem<weights>(kMostW)) != LLMFA_OK) return rc;
+  return launch_after(weights, static_cast<unsigned>(2 * sms), 8 * 32, sizeof(WSmem) + prefix, st, p);
+}
+
 }  // namespace
 
 extern "C" {
@@ -143,14 +268,11 @@ int llmfa_kv4_expand(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, v
 
 int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t heads_q, int64_t tokens,
                                        uint64_t* bytes) {
-  if (bytes == nullptr || batch < 1 || heads < 1 || heads_q < 1 || tokens < 1 ||
-      heads_q % heads != 0)
-    return LLMFA_ERR_INVALID_ARGUMENT;
-  if (batch > kKv4MaxBatch || heads_q >= (1 << 24) || tokens >= (1 << 24) ||
-      batch * heads_q >= (int64_t(1) << 31) / tokens)
-    return LLMFA_ERR_UNSUPPORTED;
-  *bytes = static_cast<uint64_t>(batch * heads_q * tokens) * 4;
-  return LLMFA_OK;
+  if (bytes == nullptr) return LLMFA_ERR_INVALID_ARGUMENT;
+  AttnShape shape;
+  const int rc = attn_shape(batch, heads, heads_q, tokens, &shape);
+  if (rc == LLMFA_OK) *bytes = attn_layout(shape).bytes;
+  return rc;
 }
 
 int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, const void* q,
@@ -174,31 +296,40 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
     p.lse_sb = lse_strides[0];
     p.lse_sh = lse_strides[1];
   }
-  uint64_t need = 0;
-  if ((rc = llmfa_kv4_attention_workspace_size(seqs->batch, cache->heads, heads_q, tokens, &need)) !=
-      LLMFA_OK)
+  AttnShape shape;
+  if ((rc = attn_shape(seqs->batch, cache->heads, heads_q, tokens, &shape)) != LLMFA_OK) return rc;
+  // the work split keeps 32-bit sums of the sequences' tiles
+  const int64_t capacity = seqs->max_pages << p.pool.page_shift;
+  if (seqs->batch * (capacity / kKv4TileTokens + 1 + kKv4UnitCost) >= (int64_t(1) << 32))
+    return LLMFA_ERR_UNSUPPORTED;
+  if (workspace == nullptr || !aligned(workspace, 16)) return LLMFA_ERR_INVALID_ARGUMENT;
+  const AttnLayout ws = attn_layout(shape);
+  if (workspace_bytes < ws.bytes) return LLMFA_ERR_INVALID_ARGUMENT;
+  int sms = 0;
+  if ((rc = device_status_ptr(&p.seqs.status)) != LLMFA_OK || (rc = device_sms(&sms)) != LLMFA_OK)
     return rc;
-  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < need)
-    return LLMFA_ERR_INVALID_ARGUMENT;
-  if ((rc = device_status_ptr(&p.seqs.status)) != LLMFA_OK) return rc;
-  const bool track = decay >= 0.f;
+  sms = sms < kMaxSms ? sms : kMaxSms;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  p.part_o = reinterpret_cast<float*>(base);
+  p.part_ml = reinterpret_cast<float2*>(base + ws.ml);
+  p.unit = reinterpret_cast<int2*>(base + ws.unit);
+  p.row_lse = decay >= 0.f ? reinterpret_cast<float*>(base + ws.row_lse) : nullptr;
   p.lse = lse;
   p.counts = counts;
-  p.row_lse = track ? static_cast<float*>(workspace) : nullptr;
   p.heads_q = static_cast<int>(heads_q);
   p.tokens = static_cast<int>(tokens);
   p.causal = causal != 0;
+  p.group = static_cast<int>(heads_q / cache->heads);
+  p.row_tiles = shape.row_tiles;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.decay = decay;
+  p.timeout_ns = wait_limit_ns();
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return by_type_and_groups(dtype, p.pool.ng, [&](auto t, auto) {
+  return by_type_and_groups(dtype, p.pool.ng, [&](auto t, auto ng) {
     using T = decltype(t);
-    kv4_simple_kernel<T><<<static_cast<unsigned>(seqs->batch * heads_q * tokens), kKv4SimpleThreads, 0,
-                           st>>>(p);
-    if ((rc = launched()) != LLMFA_OK || !track) return rc;
-    const dim3 grid(64, static_cast<unsigned>(seqs->batch * cache->heads));
-    kv4_simple_weights_kernel<T><<<grid, kKv4SimpleThreads, 0, st>>>(p);
-    return launched();
+    if (shape.nt == 1) return attn_launch<T, 1, ng.value>(p, shape, sms, st);
+    if (shape.nt == 2) return attn_launch<T, 2, ng.value>(p, shape, sms, st);
+    return attn_launch<T, 4, ng.value>(p, shape, sms, st);
   });
 }
 

@@ -36,6 +36,7 @@ struct DeviceSetup {
   int err = LLMFA_OK;
   int* status_ptr = nullptr;  // device address of g_device_status on this device
   int max_clusters = 0;
+  int sms = 0;
 };
 DeviceSetup g_setup[kMaxDevices];
 
@@ -101,6 +102,11 @@ int device_setup(int* dev_out, DeviceSetup** out) {
       return;
     }
     s.status_ptr = static_cast<int*>(sp);
+    if (cudaDeviceGetAttribute(&s.sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+      cudaGetLastError();
+      s.err = LLMFA_ERR_CUDA;
+      return;
+    }
     int n = 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2, 1, 1);
@@ -109,9 +115,7 @@ int device_setup(int* dev_out, DeviceSetup** out) {
     if (cudaOccupancyMaxActiveClusters(&n, llmfa::llm_fa_kernel_sm100<false>, &cfg) != cudaSuccess ||
         n <= 0) {
       cudaGetLastError();
-      int sms = 0;
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-      n = sms / 2;
+      n = s.sms / 2;
     }
     s.max_clusters = n > 0 ? n : 1;
   });
@@ -205,6 +209,16 @@ int llmfa::device_status_ptr(int** out) {
   if (rc == LLMFA_OK) *out = s->status_ptr;
   return rc;
 }
+
+int llmfa::device_sms(int* out) {
+  int dev = 0;
+  DeviceSetup* s = nullptr;
+  const int rc = device_setup(&dev, &s);
+  if (rc == LLMFA_OK) *out = s->sms;
+  return rc;
+}
+
+unsigned long long llmfa::wait_limit_ns() { return wait_timeout_ns(); }
 
 extern "C" {
 

@@ -65,8 +65,9 @@ _BYTE = {v: np.array([code_place(c, v)[0] for c in range(D)]) for v in (0, 1)}
 _SHIFT = np.array([code_place(c, 0)[1] for c in range(D)])
 
 
-def read(pages, table, n, page, group, h, value):
-    """fp64 [n, 128]: the first n slots of a sequence, head h. pages is uint8 numpy."""
+def read(pages, table, n, page, group, h, value, scales=False):
+    """fp64 [n, 128]: the first n slots of a sequence, head h (or each channel's scale). pages is
+    uint8 numpy."""
     i = np.arange(n)
     rows = pages[table[i // page], h]
     s = i % page
@@ -78,18 +79,21 @@ def read(pages, table, n, page, group, h, value):
     raw = np.ascontiguousarray(np.take_along_axis(rows, at, 1)).view(np.uint16).astype(np.uint32) << 16
     pair = raw.view(np.float32).astype(np.float64).reshape(n, ng, 2)
     grp = np.arange(D) // group
+    if scales:
+        return pair[:, grp, 0]
     with np.errstate(invalid="ignore"):
         return pair[:, grp, 0] * (code.astype(np.float64) - pair[:, grp, 1])
 
 
 def attention(q, pages, table, lengths, counts, *, page, group, heads, causal=True, scale=None):
-    """(o, lse, weights, magnitude, spread), fp64: o, magnitude [B, T, Hq, 128], lse [B, Hq, T],
-    weights a list of [n, heads]. magnitude is the sum of w |v|, spread the largest sum of |q k|
-    * scale of any row and key: what rounding errors are relative to. Rows past a count are NaN."""
+    """(o, lse, weights, magnitude, step, spread), fp64: o, magnitude, step [B, T, Hq, 128], lse
+    [B, Hq, T], weights a list of [n, heads]. magnitude is the sum of w |v|, step that of w *
+    value scale, spread the largest sum of |q k| * scale of any row and key: what rounding errors
+    are relative to. Rows past a count are NaN."""
     q = q.double().cpu().numpy()
     B, T, Hq, _ = q.shape
     scale = 1.0 / math.sqrt(D) if scale is None else scale
-    o, mag = np.full(q.shape, np.nan), np.zeros(q.shape)
+    o, mag, step = np.full(q.shape, np.nan), np.zeros(q.shape), np.zeros(q.shape)
     lse, weights, spread = np.full((B, Hq, T), np.nan), [], 0.0
     for b in range(B):
         n, c = int(lengths[b]), int(counts[b])
@@ -97,6 +101,7 @@ def attention(q, pages, table, lengths, counts, *, page, group, heads, causal=Tr
         for h in range(heads):
             k = read(pages, table[b], n, page, group, h, 0)
             v = read(pages, table[b], n, page, group, h, 1)
+            vs = read(pages, table[b], n, page, group, h, 1, scales=True)
             for i in range(c):
                 m = max(0, n - (c - 1 - i)) if causal else n
                 for hq in range(h * (Hq // heads), (h + 1) * (Hq // heads)):
@@ -111,11 +116,12 @@ def attention(q, pages, table, lengths, counts, *, page, group, heads, causal=Tr
                         lse[b, hq, i] = top + np.log(e.sum())
                         o[b, i, hq] = w @ v[:m]
                         mag[b, i, hq] = w @ np.abs(v[:m])
+                        step[b, i, hq] = w @ vs[:m]
                         s = (np.abs(k[:m]) @ np.abs(q[b, i, hq])).max() * scale
                     spread = max(spread, s) if np.isfinite(s) else spread
                     got[:m, h] += w
         weights.append(got)
-    return o, lse, weights, mag, spread
+    return o, lse, weights, mag, step, spread
 
 
 def select(weights, positions, table, n, *, page, keep, recent, seen, h):

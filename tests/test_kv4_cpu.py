@@ -24,16 +24,17 @@ def L():
     return _lib.lib()
 
 
-def test_index_arithmetic_and_bad_pages(tmp_path):
-    """tests/csrc/test_kv4_layout.cu runs the kernels' index functions as host code: every byte of
-    a page belongs to one code or pair, slots outside the table and ids outside the pool have no
-    page, offsets pass 32 bits."""
+@pytest.mark.parametrize("name", ["test_kv4_layout", "test_kv4_plan"])
+def test_index_arithmetic_as_host_code(tmp_path, name):
+    """tests/csrc/*.cu run the kernels' index functions as host code. Layout: every block of a
+    page is its own, slots outside the table and ids outside the pool have no page, offsets pass
+    32 bits. Plan: every tile is in exactly one CTA's share, and a cut unit's pieces are found."""
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     if not Path(nvcc).exists():
         pytest.skip("nvcc not available")
-    exe = tmp_path / "test_kv4_layout"
+    exe = tmp_path / name
     subprocess.run([nvcc, "-std=c++17", "-O1", "-gencode", "arch=compute_100a,code=sm_100a",
-                    "-o", str(exe), str(HERE / "csrc" / "test_kv4_layout.cu")],
+                    "-o", str(exe), str(HERE / "csrc" / f"{name}.cu")],
                    check=True, capture_output=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert out.returncode == 0, out.stdout + out.stderr
