@@ -86,7 +86,7 @@ int64_t quant_blocks(int64_t rows) {
   return (rows * kKv4RowThreads + kKv4QuantThreads - 1) / kKv4QuantThreads;
 }
 
-// Rows of a key head, cut into tiles of 8 nt: the least padding of 8, 16 or 32.
+// Rows of a key head, cut into tiles of 8 nt: the fewest tiles, then the least padding.
 struct AttnShape {
   int64_t batch, heads, heads_q, tokens;
   int nt, row_tiles;
@@ -100,7 +100,7 @@ int attn_shape(int64_t batch, int64_t heads, int64_t heads_q, int64_t tokens, At
       batch * heads_q >= (int64_t(1) << 31) / tokens)
     return LLMFA_ERR_UNSUPPORTED;
   const int64_t rows = tokens * (heads_q / heads);
-  const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
   const int64_t tiles = (rows + 8 * nt - 1) / (8 * nt);
   *s = AttnShape{batch, heads, heads_q, tokens, nt, static_cast<int>(tiles), batch * heads * tiles};
   return LLMFA_OK;
@@ -118,12 +118,18 @@ struct AttnConfig<2> {
   static constexpr int kWarps = 12, kStages = 2, kCtas = 1;
 };
 template <>
+struct AttnConfig<3> {
+  static constexpr int kWarps = 8, kStages = 3, kCtas = 1;
+};
+template <>
 struct AttnConfig<4> {
   static constexpr int kWarps = 8, kStages = 3, kCtas = 1;
 };
 
 int attn_ctas(int nt, int sms) {
-  return sms * (nt == 1 ? AttnConfig<1>::kCtas : nt == 2 ? AttnConfig<2>::kCtas : AttnConfig<4>::kCtas);
+  constexpr int per_sm[] = {AttnConfig<1>::kCtas, AttnConfig<2>::kCtas, AttnConfig<3>::kCtas,
+                            AttnConfig<4>::kCtas};
+  return sms * per_sm[nt - 1];
 }
 
 struct AttnLayout {  // byte offsets in the workspace; partial outputs come first
@@ -329,6 +335,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
     using T = decltype(t);
     if (shape.nt == 1) return attn_launch<T, 1, ng.value>(p, shape, sms, st);
     if (shape.nt == 2) return attn_launch<T, 2, ng.value>(p, shape, sms, st);
+    if (shape.nt == 3) return attn_launch<T, 3, ng.value>(p, shape, sms, st);
     return attn_launch<T, 4, ng.value>(p, shape, sms, st);
   });
 }

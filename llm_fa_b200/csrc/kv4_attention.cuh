@@ -4,28 +4,29 @@
 // For a key head the rows are its new tokens x query heads, in tiles of 8 NT.
 // A warp takes 32 tokens at a time:
 //
-//   S^T[token, row] = K q^T     mma m16n8k16, A = key codes, B = queries
-//   x = (S - zero * sum(q)) * scale * row factor      (log2 units, per group)
+//   S^T[token, row] = (K - zero) q^T   mma m16n8k16, A = key codes, B = queries
+//   x = S * scale * row factor         (log2 units, a sum over the groups)
 //   p = 2^(x - m), m the row's running maximum
-//   O^T[channel, row] += V^T w,  A = value codes, B = w = p * value scale
-//   Z[row] += zero * w          O is O^T - Z at the end
+//   O^T[channel, row] += (V - zero)^T w,   A = value codes, w = p * value scale
 //
-// so scales and zeros touch the few scores, never the 128 channels, and the
-// rows, not the tokens, are the narrow side of the instruction. tcgen05 would
-// pad the rows to 64 or more, and its operands would have to be written out to
-// shared memory in 16 bits first, four times the bytes that arrive.
+// so scales touch the few scores, never the 128 channels, and the rows, not
+// the tokens, are the narrow side of the instruction. tcgen05 would pad the
+// rows to 64 or more, and its operands would have to be written out to shared
+// memory in 16 bits first, four times the bytes that arrive.
 //
-// Codes become fp16 by one AND: a nibble u in bits 0-3 is the subnormal u *
-// 2^-24, in bits 4-7 u * 2^-20 (mma takes fp16 subnormals exactly); 8 codes
-// cost 4 ANDs and a shift. The factor 16 of the odd nibbles is taken out of
-// the query fragment for keys, of the output row for values. Products of codes
-// with 11-bit numbers are exact in fp32.
+// Codes become fp16 integers by one LOP3 and one HFMA2 a pair: a nibble u in
+// bits 0-3 of a half, or'ed with 0x6400, is 1024 + u, in bits 4-7 it is 1024 +
+// 16 u; taking off 1024 + zero (after a multiplication with 1/16 for the
+// latter: 64 + zero) leaves u - zero exactly. Its products with 11-bit numbers
+// are exact in fp32.
 //
 // Roundings to 16 bits: q is scaled by a power of two per row so that its
-// largest element is near 2^13 (bf16 and fp16 values stay exact down to 2^-33
+// largest element is near 2^13 (bf16 and fp16 values stay exact down to 2^-37
 // of it); w is fp16, 11 bits, scaled by a power of two per group so that the
 // largest value scale seen so far is in [1/2, 1): the running maximum of the
-// softmax, once more, for the scales. Sums, maxima and outputs are fp32.
+// softmax, once more, for the scales. For fp16 outputs, whose own rounding is
+// no coarser, w's remainder is kept in a second fp16 and multiplied too. Sums,
+// maxima and outputs are fp32.
 //
 // The row maximum is lazy: p may reach 2^kKv4Slack before O is rescaled, so a
 // tile needs one vote instead of a reduction over lanes.
@@ -35,6 +36,8 @@
 // lane issues them, the warp waits on its own barrier, and warps meet only
 // where a unit ends and their parts are joined.
 #pragma once
+#include <type_traits>
+
 #include "kv4_plan.cuh"
 #include "kv4_quant.cuh"
 #include "ptx.cuh"
@@ -66,7 +69,6 @@ constexpr int kKv4WeightBits = 8;  // w < 2^(kKv4WeightBits + kKv4Slack)
 constexpr int kStatusTimeout = 0x1000;  // + wait site: a bounded wait gave up
 constexpr int kSiteKv4Tile = 13;
 constexpr unsigned long long kKv4DrainNs = 1000000;
-constexpr uint32_t kNibbleLo = 0x000f000fu, kNibbleHi = 0x00f000f0u;
 
 // ---------------------------------------------------------------- instructions
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -111,6 +113,46 @@ __device__ __forceinline__ void ld_pairs(uint32_t addr, uint32_t (&w)[NG]) {
   }
 }
 
+// ---------------------------------------------------------------- codes
+// Two halves of 1024 + u (nibble 0 of each half of w), or of 1024 + 16 u (nibble 1).
+__device__ __forceinline__ uint32_t nibbles_lo(uint32_t w) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t nibbles_hi(uint32_t w) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// a / 16 - b
+__device__ __forceinline__ uint32_t sixteenth_minus(uint32_t a, uint32_t minus_b) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0x2c002c00u), "r"(minus_b));
+  return r;
+}
+// What is taken off the two kinds: 1024 + zero, and -(64 + zero).
+struct Kv4Zero {
+  uint32_t lo, hi;
+};
+// Of two tokens' pairs, one in each half. A pair read as fp32 is its zero, an integer, plus less
+// than 1/16 (the scale's bits are the low end of the mantissa); adding 2^23 + 0x6400 leaves 0x6400
+// + zero, the fp16 number 1024 + zero, in the low half.
+__device__ __forceinline__ Kv4Zero kv4_zero(uint32_t pair_a, uint32_t pair_b) {
+  const uint32_t a = __float_as_uint(__uint_as_float(pair_a) + 8414208.f);
+  const uint32_t b = __float_as_uint(__uint_as_float(pair_b) + 8414208.f);
+  Kv4Zero z;
+  z.lo = __byte_perm(a, b, 0x5410);
+  z.hi = sub_f16x2(0x63806380u, z.lo);  // 960 - (1024 + zero)
+  return z;
+}
+__device__ __forceinline__ float kv4_scale(uint32_t pair) { return __uint_as_float(pair << 16); }
+
 // ---------------------------------------------------------------- query rows
 // Row r of a key head is new token r / group, query head r % group.
 struct Kv4Row {
@@ -126,7 +168,6 @@ __device__ __forceinline__ Kv4Row kv4_row(const Kv4AttnParams& p, int h, int c, 
 template <int NT, int NG>
 struct Kv4Queries {
   uint2 frag[8][NT][32];    // B fragments of the 8 steps of 16 channels
-  float sum[NG][8 * NT];    // sum of a group's queries, * 2^-24
   float factor[8 * NT];     // of a score
   int limit[8 * NT];        // slots that the row sees
 };
@@ -166,30 +207,18 @@ __device__ __forceinline__ void kv4_load_queries(const Kv4AttnParams& p, Kv4Quer
   // 2^e brings the largest element to [2^13, 2^14)
   const int e = min(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126);
   const float up = bad == 0.f ? __int_as_float((e + 127) << 23) : 0.f;
-  float sum[NG] = {};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    float y[8];
+    uint32_t y[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float v = (bad == 0.f ? x[j][k] : 0.f) * up * (k & 1 ? 0.0625f : 1.f);
-      y[k] = __half2float(__float2half_rn(v));
-      sum[j * NG / 4] += y[k] * (k & 1 ? 16.f : 1.f);
-    }
-    qs.frag[2 * j][nt][lane] = make_uint2(Kv4Type<__half>::pack(y[0], y[4]),
-                                          Kv4Type<__half>::pack(y[1], y[5]));
-    qs.frag[2 * j + 1][nt][lane] = make_uint2(Kv4Type<__half>::pack(y[2], y[6]),
-                                              Kv4Type<__half>::pack(y[3], y[7]));
-  }
-#pragma unroll
-  for (int k = 0; k < NG; ++k) {
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], d);
-    if (cc == 0) qs.sum[k][8 * nt + g] = sum[k] * 0x1p-24f;
+    for (int k = 0; k < 4; ++k)
+      y[k] = bad == 0.f ? Kv4Type<__half>::pack(x[j][k] * up, x[j][k + 4] * up) : 0u;
+    qs.frag[2 * j][nt][lane] = make_uint2(y[0], y[1]);
+    qs.frag[2 * j + 1][nt][lane] = make_uint2(y[2], y[3]);
   }
   if (cc == 0) {
     qs.factor[8 * nt + g] =
-        bad == 0.f ? ldexpf(p.scale_log2, 24 - e) : __int_as_float(0x7fc00000);
+        bad == 0.f ? ldexpf(p.scale_log2, -e) : __int_as_float(0x7fc00000);
     qs.limit[8 * nt + g] = row.live ? kv4_visible(n, c, row.i, p.causal) : 0;
   }
 }
@@ -238,51 +267,59 @@ struct Kv4Ring {
 
 // Walks the tiles of a CTA's segments that belong to one warp, ahead of the
 // computation, and finds their blocks. Tiles go round the warps.
+// What is needed once a segment stays in shared memory: registers are short.
 template <int WARPS>
 struct Kv4Loader {
-  Kv4Segment seg;
-  int tile, n;
-  int row_tiles;
+  Kv4Segment* seg;       // this warp's, in shared memory
+  const int32_t* table;  // of the segment's sequence
+  int tile, hi, n, h;
   bool more;
-  long long page;  // of this lane's block of the tile
+  int page;  // of this lane's block of the tile, or -1
 
-  __device__ __forceinline__ void find(const Kv4AttnParams& p, const Kv4Split& s, int warp,
-                                       bool fresh) {
-    if (fresh && more) {
-      tile = seg.lo + warp;
-      n = kv4_clamp(p.seqs.lengths[seg.b], kv4_capacity(p.pool, p.seqs));
-    }
-    while (more && tile >= seg.hi) {
-      more = seg.next(s);
-      if (more) {
-        tile = seg.lo + warp;
-        n = kv4_clamp(p.seqs.lengths[seg.b], kv4_capacity(p.pool, p.seqs));
-      }
+  __device__ __forceinline__ int slot() const {
+    return tile * kKv4TileTokens + (threadIdx.x & 31) * kKv4Block;
+  }
+  __device__ __forceinline__ void enter(const Kv4AttnParams& p, const Kv4Segment& s, int warp,
+                                        int row_tiles) {
+    if ((threadIdx.x & 31) == 0) *seg = s;
+    __syncwarp();
+    tile = s.lo + warp;
+    hi = s.hi;
+    n = kv4_clamp(p.seqs.lengths[s.b], kv4_capacity(p.pool, p.seqs));
+    table = p.seqs.table + s.b * p.seqs.table_stride;
+    h = s.i / row_tiles;
+  }
+  __device__ __forceinline__ void find(const Kv4AttnParams& p, const Kv4Split& split, int warp,
+                                       int row_tiles) {
+    while (more && tile >= hi) {
+      Kv4Segment s = *seg;
+      __syncwarp();
+      more = s.next(split);
+      if (more) enter(p, s, warp, row_tiles);
     }
     page = -1;
-    const int lane = threadIdx.x & 31;
-    const long long slot = static_cast<long long>(tile) * kKv4TileTokens + lane * kKv4Block;
-    if (more && lane < kKv4TokenBlocks && slot < n) {
-      page = kv4_page(p.pool, p.seqs, seg.b, slot);
-      if (page < 0) kv4_report(p.seqs, kStatusKv4BadPage);
+    if (more && (threadIdx.x & 31) < kKv4TokenBlocks && slot() < n) {  // n is inside the table
+      page = table[slot() >> p.pool.page_shift];
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.pool.num_pages)) {
+        page = -1;
+        kv4_report(p.seqs, kStatusKv4BadPage);
+      }
     }
   }
-  __device__ __forceinline__ void start(const Kv4AttnParams& p, const Kv4Split& s, int cta,
-                                        int warp, int tiles_a_head) {
-    row_tiles = tiles_a_head;
-    more = seg.first(s, cta);
-    find(p, s, warp, true);
+  __device__ __forceinline__ void start(const Kv4AttnParams& p, const Kv4Split& split, int cta,
+                                        int warp, int row_tiles) {
+    Kv4Segment s;
+    more = s.first(split, cta);
+    if (more) enter(p, s, warp, row_tiles);
+    find(p, split, warp, row_tiles);
   }
   template <typename Ring>
-  __device__ __forceinline__ void issue(const Kv4AttnParams& p, const Kv4Split& s, Ring& ring,
-                                        int warp) {
+  __device__ __forceinline__ void issue(const Kv4AttnParams& p, const Kv4Split& split, Ring& ring,
+                                        int warp, int row_tiles) {
     if (!more) return;
-    const long long slot =
-        static_cast<long long>(tile) * kKv4TileTokens + (threadIdx.x & 31) * kKv4Block;
-    ring.issue(page >= 0 ? p.pool.pages + kv4_block_offset(p.pool, page, seg.i / row_tiles, slot)
-                         : nullptr);
+    ring.issue(page >= 0 ? p.pool.pages + kv4_block_offset(p.pool, page, h, slot()) : nullptr);
     tile += WARPS;
-    find(p, s, warp, false);
+    find(p, split, warp, row_tiles);
   }
 };
 
@@ -313,44 +350,230 @@ __device__ __forceinline__ void kv4_prefix(const Kv4AttnParams& p, uint32_t* pre
   }
 }
 
-// Key codes of 16 tokens times the query rows: the raw scores of tokens a (row
-// g of the instruction) and a + 8, then x, in log2 units without the row factor.
+// Key codes of 16 tokens times the query rows: x of tokens a (row g of the
+// instruction) and a + 8, in log2 units but for the row factor.
 template <int NT, int NG, typename Frag>
-__device__ __forceinline__ void kv4_scores(uint32_t block, int tok, const uint32_t (&pa)[NG],
-                                           const uint32_t (&pb)[NG], const float (&qsum)[NG][NT][2],
-                                           Frag frag, float (&x)[NT][4]) {
-  const int cc = threadIdx.x & 3;
-  const uint4 va = ptx::ld_shared_v4(block + tok * kKv4RowBytes + cc * 16);
-  const uint4 vb = ptx::ld_shared_v4(block + (tok + 8) * kKv4RowBytes + cc * 16);
+__device__ __forceinline__ void kv4_scores(uint32_t block, int tok, Frag frag, float (&x)[NT][4]) {
+  const uint32_t row = block + tok * kKv4RowBytes + (threadIdx.x & 3) * 16;
+  const uint4 va = ptx::ld_shared_v4(row), vb = ptx::ld_shared_v4(row + 8 * kKv4RowBytes);
+  const uint32_t pairs = block + kKv4Block * kKv4RowBytes + tok * 4 * NG;
+  uint32_t pa[NG], pb[NG];
+  ld_pairs<NG>(pairs, pa);
+  ld_pairs<NG>(pairs + 8 * 4 * NG, pb);
   const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
-  float raw[NT][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j % (4 / NG) == 0) {
+  for (int grp = 0; grp < NG; ++grp) {
+    const Kv4Zero za = kv4_zero(pa[grp], pa[grp]), zb = kv4_zero(pb[grp], pb[grp]);
+    float raw[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) raw[nt][k] = 0.f;
-    }
+      for (int k = 0; k < 4; ++k) raw[nt][k] = 0.f;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const uint32_t ua = wa[j] >> (8 * half), ub = wb[j] >> (8 * half);
+    for (int j = grp * 4 / NG; j < (grp + 1) * 4 / NG; ++j) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const uint2 f = frag(2 * j + half, nt);
-        mma_f16(raw[nt], ua & kNibbleLo, ub & kNibbleLo, ua & kNibbleHi, ub & kNibbleHi, f.x, f.y);
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t ua = wa[j] >> (8 * half), ub = wb[j] >> (8 * half);
+        const uint32_t a0 = sub_f16x2(nibbles_lo(ua), za.lo), a1 = sub_f16x2(nibbles_lo(ub), zb.lo);
+        const uint32_t a2 = sixteenth_minus(nibbles_hi(ua), za.hi);
+        const uint32_t a3 = sixteenth_minus(nibbles_hi(ub), zb.hi);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint2 f = frag(2 * j + half, nt);
+          mma_f16(raw[nt], a0, a1, a2, a3, f.x, f.y);
+        }
       }
     }
-    if ((j + 1) % (4 / NG) == 0) {
-      const int grp = j * NG / 4;
-      const float2 a = kv4_scale_zero(pa[grp]), b = kv4_scale_zero(pb[grp]);
+    const float sa = kv4_scale(pa[grp]), sb = kv4_scale(pb[grp]);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float sc = k < 2 ? sa : sb;
+        x[nt][k] = grp == 0 ? raw[nt][k] * sc : fmaf(raw[nt][k], sc, x[nt][k]);
+      }
+  }
+}
+
+// A warp's running sums over the tokens of a segment.
+template <int NT, int NG>
+struct Kv4State {
+  float o[8][NT][4];  // m-tile i: channels 32 (i / 2) + 4 g + 2 (i % 2) and + 1, rows 2c, 2c + 1
+  float m[NT][2], l[NT][2];
+  int top[NG];        // exponent (biased) that the value scales seen so far stay within
+};
+
+// One tile of 32 tokens. RAGGED: some row does not see all of it (or a block is
+// missing): `blocks` says which are here, `limit` what each row sees, n what
+// the sequence holds, all counted from the tile's first slot.
+template <typename T, int NT, int NG, bool RAGGED, typename Frag>
+__device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, int tok, Frag frag,
+                                         const float (&factor)[NT][2], uint32_t blocks,
+                                         const int* limit, int slot0, int n) {
+  constexpr bool kTwo = std::is_same<T, __half>::value;  // w in two halves
+  constexpr int kBlockBytes = kv4_block_bytes(NG);
+  const int lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
+  float x[2][NT][4];
+  uint32_t pv[2][2][NG];  // value pairs of tokens tok and tok + 8 of both blocks
+  uint32_t seen = 0;      // bit ((2 s + u) * NT + nt) * 2 + k
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const uint32_t block = tile + s * kBlockBytes;
+    kv4_scores<NT, NG>(block, tok, frag, x[s]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      ld_pairs<NG>(block + kv4_half_bytes(NG) + kKv4Block * kKv4RowBytes + (tok + 8 * u) * 4 * NG,
+                   pv[s][u]);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[s][nt][k] *= factor[nt][k & 1];
+    if constexpr (RAGGED) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int slot = slot0 + 16 * s + tok + 8 * u;
+        const bool here = ((blocks >> s) & 1u) != 0;
+        if (!here || slot >= n) {
+#pragma unroll
+          for (int grp = 0; grp < NG; ++grp) pv[s][u][grp] = 0;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (here && slot < limit[8 * nt + 2 * cc + k]) seen |= 1u << (((2 * s + u) * NT + nt) * 2 + k);
+            else x[s][nt][2 * u + k] = -INFINITY;
+          }
+      }
+    }
+  }
+
+  // maxima and value scales: a vote decides whether anything has to be rescaled
+  bool grow = false;
+  float big[NG];
+#pragma unroll
+  for (int grp = 0; grp < NG; ++grp) {
+    big[grp] = fmaxf(fmaxf(kv4_scale(pv[0][0][grp]), kv4_scale(pv[0][1][grp])),
+                     fmaxf(kv4_scale(pv[1][0][grp]), kv4_scale(pv[1][1][grp])));
+    grow |= big[grp] >= __int_as_float((st.top[grp] + 1) << 23);
+  }
+  float mx[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      mx[nt][k] = fmaxf(fmaxf(x[0][nt][k], x[0][nt][2 + k]), fmaxf(x[1][nt][k], x[1][nt][2 + k]));
+      grow |= mx[nt][k] > st.m[nt][k] + kKv4Slack;
+    }
+  if (__any_sync(0xffffffffu, grow)) {
+    float down[NG];
+#pragma unroll
+    for (int grp = 0; grp < NG; ++grp) {
+      // an infinite scale (exponent 255) is no scale of the format: it may overflow
+      const int e = max(st.top[grp],
+                        __reduce_max_sync(0xffffffffu, min(__float_as_int(big[grp]) >> 23, 254)));
+      const int shift = st.top[grp] - e;  // 2^shift, 0 below fp32's range
+      down[grp] = shift < -126 ? 0.f : __int_as_float((shift + 127) << 23);
+      st.top[grp] = e;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float v = mx[nt][k];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+        const float mn = fmaxf(st.m[nt][k], v);
+        const float a = st.m[nt][k] == -INFINITY ? 1.f : ptx::ex2_mufu(st.m[nt][k] - mn);
+        st.m[nt][k] = mn;
+        st.l[nt][k] *= a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          st.o[i][nt][k] *= a * down[i * NG / 8];
+          st.o[i][nt][2 + k] *= a * down[i * NG / 8];
+        }
+      }
+  }
+
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    // p, and w = p * value scale * 2^(weight bits - top), as the product's B operand
+    uint32_t w[NG][NT][2], rest[kTwo ? NG : 1][NT][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float f[NG];
+#pragma unroll
+      for (int grp = 0; grp < NG; ++grp)
+        f[grp] = kv4_scale(pv[s][u][grp]) *
+                 __int_as_float((127 + 127 + kKv4WeightBits - 1 - st.top[grp]) << 23);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        float pr[2];
+        bool see[2] = {true, true};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 sz = k < 2 ? a : b;
-          const float t = fmaf(-sz.y, qsum[grp][nt][k & 1], raw[nt][k]);
-          x[nt][k] = grp == 0 ? t * sz.x : fmaf(t, sz.x, x[nt][k]);
+        for (int k = 0; k < 2; ++k) {
+          pr[k] = ptx::ex2_mufu(x[s][nt][2 * u + k] - st.m[nt][k]);
+          if constexpr (RAGGED) {
+            see[k] = ((seen >> (((2 * s + u) * NT + nt) * 2 + k)) & 1u) != 0;
+            if (!see[k]) pr[k] = 0.f;
+          }
+          st.l[nt][k] += pr[k];
+        }
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          // an unseen token may hold a NaN scale
+          const float w0 = see[0] ? pr[0] * f[grp] : 0.f, w1 = see[1] ? pr[1] * f[grp] : 0.f;
+          const uint32_t h2 = Kv4Type<__half>::pack(w0, w1);
+          w[grp][nt][u] = transpose8x8(h2);
+          if constexpr (kTwo) {
+            const float2 back = Kv4Type<__half>::unpack(h2);
+            rest[grp][nt][u] = transpose8x8(Kv4Type<__half>::pack(w0 - back.x, w1 - back.y));
+          }
+        }
+      }
+    }
+    // Columns 2c, 2c + 1 of the values' operand are tokens c, c + 4 of the block, 2c + 8, 2c + 9
+    // tokens c + 8, c + 12; a lane holds 16 channels of each, 4 of every 32.
+    const uint32_t half = tile + s * kBlockBytes + kv4_half_bytes(NG);
+    uint2 v[4];
+    Kv4Zero z[NG][2];
+    {
+      uint32_t pz[4][NG];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = ld_shared_v2(half + (cc + 4 * i) * kKv4RowBytes + g * 8);
+        ld_pairs<NG>(half + kKv4Block * kKv4RowBytes + (cc + 4 * i) * 4 * NG, pz[i]);
+        if constexpr (RAGGED) {
+          if (((blocks >> s) & 1u) == 0 || slot0 + 16 * s + cc + 4 * i >= n) {
+#pragma unroll
+            for (int grp = 0; grp < NG; ++grp) pz[i][grp] = 0;
+          }
+        }
+      }
+#pragma unroll
+      for (int grp = 0; grp < NG; ++grp) {
+        z[grp][0] = kv4_zero(pz[0][grp], pz[1][grp]);
+        z[grp][1] = kv4_zero(pz[2][grp], pz[3][grp]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // channels 32 k + 4 g ..
+      const int grp = k * NG / 4;
+      const uint32_t sel = (k & 1) ? 0x7632u : 0x5410u;
+      const uint32_t ra = k < 2 ? __byte_perm(v[0].x, v[1].x, sel) : __byte_perm(v[0].y, v[1].y, sel);
+      const uint32_t rb = k < 2 ? __byte_perm(v[2].x, v[3].x, sel) : __byte_perm(v[2].y, v[3].y, sel);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t ua = ra >> (8 * h), ub = rb >> (8 * h);
+        const uint32_t a0 = sub_f16x2(nibbles_lo(ua), z[grp][0].lo);
+        const uint32_t a1 = sixteenth_minus(nibbles_hi(ua), z[grp][0].hi);
+        const uint32_t a2 = sub_f16x2(nibbles_lo(ub), z[grp][1].lo);
+        const uint32_t a3 = sixteenth_minus(nibbles_hi(ub), z[grp][1].hi);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma_f16(st.o[2 * k + h][nt], a0, a1, a2, a3, w[grp][nt][0], w[grp][nt][1]);
+          if constexpr (kTwo)
+            mma_f16(st.o[2 * k + h][nt], a0, a1, a2, a3, rest[grp][nt][0], rest[grp][nt][1]);
         }
       }
     }
@@ -384,6 +607,8 @@ struct Kv4AttnSmem {
   float join[WARPS][kJoinBlocks][8 * NT][kJoinRow];
   float2 ml[WARPS][8 * NT];
   Kv4Queries<NT, NG> q;
+  Kv4Split split;
+  Kv4Segment seg[WARPS];
   uint64_t bar[WARPS][STAGES];
 };
 
@@ -402,19 +627,20 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
     ptx::fence_mbar_init();
   }
   kv4_prefix<kThreads>(p, prefix);
+  if (threadIdx.x == 0) sm.split = kv4_split(prefix, p.seqs.batch, p.pool.heads * p.row_tiles, p.ctas);
   __syncthreads();
-  const Kv4Split split = kv4_split(prefix, p.seqs.batch, p.pool.heads * p.row_tiles, p.ctas);
+  const Kv4Split& split = sm.split;
   const int cta = blockIdx.x;
   if (cta >= split.parts) return;
 
   Kv4Ring<STAGES, kv4_block_bytes(NG)> ring{ptx::smem_u32(sm.ring[warp]),
                                             ptx::smem_u32(sm.bar[warp]), 0, 0, 0};
   Kv4Loader<WARPS> loader;
+  loader.seg = &sm.seg[warp];
   loader.start(p, split, cta, warp, p.row_tiles);
-  for (int s = 0; s < STAGES; ++s) loader.issue(p, split, ring, warp);
+  for (int s = 0; s < STAGES; ++s) loader.issue(p, split, ring, warp, p.row_tiles);
 
-  // matrix rows g and g + 8 are tokens tok and tok + 8 of a block; columns 2c, 2c + 8 of the
-  // values' operand tokens c, c + 8, columns 2c + 1, 2c + 9 tokens c + 4, c + 12
+  // rows g and g + 8 of the keys' operand are tokens tok and tok + 8 of a block
   const int tok = (g >> 1) + 4 * (g & 1);
   unsigned long long limit_ns = p.timeout_ns;
 
@@ -437,36 +663,25 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
       if constexpr (NT <= 2) return qf[s][nt];
       else return sm.q.frag[s][nt][lane];
     };
-    float qsum[NG][NT][2], factor[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int grp = 0; grp < NG; ++grp) qsum[grp][nt][k] = sm.q.sum[grp][8 * nt + 2 * cc + k];
-        factor[nt][k] = sm.q.factor[8 * nt + 2 * cc + k];
-      }
-    // slots below `all` are seen by every live row
-    const int all = p.causal ? kv4_visible(n, c, r0 / p.group, true) : n;
-
-    float o[8][NT][4], z[NG][NT][2], m[NT][2], l[NT][2];
-    int top[NG];  // exponent of the largest value scale so far, biased
+    Kv4State<NT, NG> st;
+    float factor[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.f;
+        for (int k = 0; k < 4; ++k) st.o[i][nt][k] = 0.f;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        m[nt][k] = -INFINITY;
-        l[nt][k] = 0.f;
-#pragma unroll
-        for (int grp = 0; grp < NG; ++grp) z[grp][nt][k] = 0.f;
+        st.m[nt][k] = -INFINITY;
+        st.l[nt][k] = 0.f;
+        factor[nt][k] = sm.q.factor[8 * nt + 2 * cc + k];
       }
     }
 #pragma unroll
-    for (int grp = 0; grp < NG; ++grp) top[grp] = 127 - 100;
+    for (int grp = 0; grp < NG; ++grp) st.top[grp] = 127 - 100;
+    // slots below `all` are seen by every live row
+    const int all = p.causal ? kv4_visible(n, c, r0 / p.group, true) : n;
 
     for (int t = seg.lo + warp; t < seg.hi; t += WARPS) {
       uint32_t blocks = ring.blocks();
@@ -477,166 +692,13 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
         loader.more = false;
         blocks = 0;
       }
-      const uint32_t tile = ring.tile();
       const int slot0 = t * kKv4TileTokens;
-      // a tile that some row does not see whole: past a limit, or without its blocks
-      const bool ragged = slot0 + kKv4TileTokens > all || blocks != 3u;
-
-      float x[2][NT][4];
-      uint32_t pv[2][2][NG];  // value pairs of tokens tok and tok + 8 of both blocks
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const uint32_t block = tile + s * kv4_block_bytes(NG);
-        const uint32_t pairs = block + kKv4Block * kKv4RowBytes;
-        uint32_t pk[2][NG];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          ld_pairs<NG>(pairs + (tok + 8 * u) * 4 * NG, pk[u]);
-          ld_pairs<NG>(pairs + kv4_half_bytes(NG) + (tok + 8 * u) * 4 * NG, pv[s][u]);
-        }
-        kv4_scores<NT, NG>(block, tok, pk[0], pk[1], qsum, frag, x[s]);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x[s][nt][k] *= factor[nt][k & 1];
-      }
-      uint32_t seen = 0xffffffffu;  // bit (2 s + u) * 2 NT + 2 nt + k
-      if (ragged) {
-        seen = 0;
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int slot = slot0 + 16 * s + tok + 8 * u;
-            const bool here = ((blocks >> s) & 1u) != 0;
-            bool any = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const bool see = here && slot < sm.q.limit[8 * nt + 2 * cc + k];
-                any |= see;
-                if (see) seen |= 1u << ((2 * s + u) * 2 * NT + 2 * nt + k);
-                else x[s][nt][2 * u + k] = -INFINITY;
-              }
-            if (!any) {
-#pragma unroll
-              for (int grp = 0; grp < NG; ++grp) pv[s][u][grp] = 0;
-            }
-          }
-      }
-
-      // maxima and value scales: a vote decides whether anything has to be rescaled
-      bool grow = false;
-      int ex[NG];
-#pragma unroll
-      for (int grp = 0; grp < NG; ++grp) {
-        ex[grp] = 0;
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int e = static_cast<int>((pv[s][u][grp] >> 7) & 255u);
-            ex[grp] = max(ex[grp], e == 255 ? 0 : e);
-          }
-        grow |= ex[grp] > top[grp];
-      }
-      float mx[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          mx[nt][k] = fmaxf(fmaxf(x[0][nt][k], x[0][nt][2 + k]), fmaxf(x[1][nt][k], x[1][nt][2 + k]));
-          grow |= mx[nt][k] > m[nt][k] + kKv4Slack;
-        }
-      if (__any_sync(0xffffffffu, grow)) {
-        float down[NG];
-#pragma unroll
-        for (int grp = 0; grp < NG; ++grp) {
-          const int e = max(top[grp], __reduce_max_sync(0xffffffffu, ex[grp]));
-          const int shift = top[grp] - e;  // 2^shift, 0 below fp32's range
-          down[grp] = shift < -126 ? 0.f : __int_as_float((shift + 127) << 23);
-          top[grp] = e;
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float v = mx[nt][k];
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-            const float mn = fmaxf(m[nt][k], v);
-            const float a = m[nt][k] == -INFINITY ? 1.f : ptx::ex2_mufu(m[nt][k] - mn);
-            m[nt][k] = mn;
-            l[nt][k] *= a;
-#pragma unroll
-            for (int grp = 0; grp < NG; ++grp) z[grp][nt][k] *= a * down[grp];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              o[i][nt][k] *= a * down[i * NG / 8];
-              o[i][nt][2 + k] *= a * down[i * NG / 8];
-            }
-          }
-      }
-
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        // p, and w = p * value scale * 2^(weight bits - top), as the product's B operand
-        uint32_t wb[NG][NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float pr[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float d = x[s][nt][2 * u + k] - m[nt][k];
-              pr[k] = ptx::ex2_mufu(d);
-              if (ragged && ((seen >> ((2 * s + u) * 2 * NT + 2 * nt + k)) & 1u) == 0) pr[k] = 0.f;
-              l[nt][k] += pr[k];
-            }
-#pragma unroll
-            for (int grp = 0; grp < NG; ++grp) {
-              const float2 sz = kv4_scale_zero(pv[s][u][grp]);
-              const float f = sz.x * __int_as_float((127 + 127 + kKv4WeightBits - 1 - top[grp]) << 23);
-              float w[2];
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                w[k] = pr[k] * f;
-                // an unseen token may hold a NaN scale
-                if (ragged && ((seen >> ((2 * s + u) * 2 * NT + 2 * nt + k)) & 1u) == 0) w[k] = 0.f;
-              }
-              const uint32_t h2 = Kv4Type<__half>::pack(w[0], w[1]);
-              const float2 back = Kv4Type<__half>::unpack(h2);
-              z[grp][nt][0] = fmaf(sz.y, back.x, z[grp][nt][0]);
-              z[grp][nt][1] = fmaf(sz.y, back.y, z[grp][nt][1]);
-              wb[grp][nt][u] = transpose8x8(h2);
-            }
-          }
-        // value codes of tokens cc, cc + 4, cc + 8, cc + 12: 16 channels a lane
-        const uint32_t vals = tile + s * kv4_block_bytes(NG) + kv4_half_bytes(NG) + g * 8;
-        uint2 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = ld_shared_v2(vals + (cc + 4 * i) * kKv4RowBytes);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {  // channels 32 k + 4 g ..
-          const uint32_t sel = (k & 1) ? 0x7632u : 0x5410u;
-          const uint32_t ra = k < 2 ? __byte_perm(v[0].x, v[1].x, sel) : __byte_perm(v[0].y, v[1].y, sel);
-          const uint32_t rb = k < 2 ? __byte_perm(v[2].x, v[3].x, sel) : __byte_perm(v[2].y, v[3].y, sel);
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t ua = ra >> (8 * half), ub = rb >> (8 * half);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint32_t* w = wb[k * NG / 4][nt];
-              mma_f16(o[2 * k + half][nt], ua & kNibbleLo, ua & kNibbleHi, ub & kNibbleLo,
-                      ub & kNibbleHi, w[0], w[1]);
-            }
-          }
-        }
-      }
+      if (slot0 + kKv4TileTokens > all || blocks != 3u)
+        kv4_tile<T, NT, NG, true>(st, ring.tile(), tok, frag, factor, blocks, sm.q.limit, slot0, n);
+      else
+        kv4_tile<T, NT, NG, false>(st, ring.tile(), tok, frag, factor, blocks, sm.q.limit, slot0, n);
       ring.release();
-      loader.issue(p, split, ring, warp);
+      loader.issue(p, split, ring, warp, p.row_tiles);
     }
 
     // ---- join the warps
@@ -644,14 +706,10 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
+        float l = st.l[nt][k];
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          l[nt][k] += __shfl_xor_sync(0xffffffffu, l[nt][k], d);
-#pragma unroll
-          for (int grp = 0; grp < NG; ++grp)
-            z[grp][nt][k] += __shfl_xor_sync(0xffffffffu, z[grp][nt][k], d);
-        }
-        if (g == 0) sm.ml[warp][8 * nt + 2 * cc + k] = make_float2(m[nt][k], l[nt][k]);
+        for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        if (g == 0) sm.ml[warp][8 * nt + 2 * cc + k] = make_float2(st.m[nt][k], l);
       }
     const Kv4Pieces pieces = kv4_pieces(split, seg.at, seg.tiles);
     const bool whole = pieces.count == 1;
@@ -664,20 +722,14 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
 #pragma unroll
       for (int kk = 0; kk < kJoin; ++kk) {
         const int k = k0 + kk, grp = k * NG / 4;
-        // 2^24 of the codes, and w's own factor, taken back
-        const float back = __int_as_float((top[grp] + 1 - kKv4WeightBits) << 23);
+        const float back = __int_as_float((st.top[grp] + 1 - kKv4WeightBits) << 23);  // w's factor
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float zz = z[grp][nt][j];
-            float4 f;
-            f.x = (o[2 * k][nt][j] * 0x1p24f - zz) * back;
-            f.y = (o[2 * k][nt][2 + j] * 0x1p20f - zz) * back;
-            f.z = (o[2 * k + 1][nt][j] * 0x1p24f - zz) * back;
-            f.w = (o[2 * k + 1][nt][2 + j] * 0x1p20f - zz) * back;
-            *reinterpret_cast<float4*>(&sm.join[warp][kk][8 * nt + 2 * cc + j][4 * g]) = f;
-          }
+          for (int j = 0; j < 2; ++j)
+            *reinterpret_cast<float4*>(&sm.join[warp][kk][8 * nt + 2 * cc + j][4 * g]) =
+                make_float4(st.o[2 * k][nt][j] * back, st.o[2 * k][nt][2 + j] * back,
+                            st.o[2 * k + 1][nt][j] * back, st.o[2 * k + 1][nt][2 + j] * back);
       }
       __syncthreads();
       // each thread 4 channels of a row, over the warps
@@ -760,6 +812,8 @@ struct Kv4WeightsSmem {
   Kv4Queries<NT, NG> q;
   float lse[8 * NT];
   int page[WARPS][STAGES][kKv4TokenBlocks];
+  Kv4Split split;
+  Kv4Segment seg[WARPS];
   uint64_t bar[WARPS][STAGES];
 };
 
@@ -777,18 +831,20 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
     ptx::fence_mbar_init();
   }
   kv4_prefix<kThreads>(p, prefix);
+  if (threadIdx.x == 0) sm.split = kv4_split(prefix, p.seqs.batch, p.pool.heads, gridDim.x);
   __syncthreads();
-  const Kv4Split split = kv4_split(prefix, p.seqs.batch, p.pool.heads, gridDim.x);
+  const Kv4Split& split = sm.split;
   const int cta = blockIdx.x;
   if (cta >= split.parts) return;
   Kv4Ring<STAGES, kv4_half_bytes(NG)> ring{ptx::smem_u32(sm.ring[warp]),
                                            ptx::smem_u32(sm.bar[warp]), 0, 0, 0};
   Kv4Loader<WARPS> loader{};
+  loader.seg = &sm.seg[warp];
   unsigned long long limit_ns = p.timeout_ns;
   auto issue = [&] {
     if (loader.more && lane < kKv4TokenBlocks)
-      sm.page[warp][ring.head % STAGES][lane] = static_cast<int>(loader.page);
-    loader.issue(p, split, ring, warp);
+      sm.page[warp][ring.head % STAGES][lane] = loader.page;
+    loader.issue(p, split, ring, warp, 1);
   };
   const int tok = (g >> 1) + 4 * (g & 1);
   for (int rt = 0; rt < p.row_tiles; ++rt) {
@@ -821,14 +877,12 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
         if constexpr (NT <= 2) return qf[s][nt];
         else return sm.q.frag[s][nt][lane];
       };
-      float qsum[NG][NT][2], factor[NT][2], lse[NT][2];
+      float factor[NT][2], lse[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int r = 8 * nt + 2 * cc + k;
-#pragma unroll
-          for (int grp = 0; grp < NG; ++grp) qsum[grp][nt][k] = sm.q.sum[grp][r];
           factor[nt][k] = sm.q.factor[r];
           lse[nt][k] = sm.lse[r];
         }
@@ -846,12 +900,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const uint32_t block = tile + s * kv4_half_bytes(NG);
-          uint32_t pk[2][NG];
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            ld_pairs<NG>(block + kKv4Block * kKv4RowBytes + (tok + 8 * u) * 4 * NG, pk[u]);
           float x[NT][4];
-          kv4_scores<NT, NG>(block, tok, pk[0], pk[1], qsum, frag, x);
+          kv4_scores<NT, NG>(block, tok, frag, x);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int slot = slot0 + 16 * s + tok + 8 * u;
