@@ -212,8 +212,9 @@ int llmfa_selftest_wait_timeout(uint32_t timeout_us, void* stream);
  * aligned, laid out in blocks of 16 tokens (16 x 64 bytes of key codes, 16 x
  * 128/group (scale, zero) pairs of bf16, then the same of values). group (32,
  * 64 or 128) channels share a pair: a code u stands for scale * (u - zero).
- * positions and weights are [num_pages][heads][page_size]: the position that a
- * token was appended at and the attention weight that it has accumulated. */
+ * positions and weights are [num_pages][heads][page_size], 16-byte aligned: the
+ * position that a token was appended at and the attention weight that it has
+ * accumulated. */
 typedef struct llmfa_kv4_cache {
   void* pages;
   int32_t* positions;

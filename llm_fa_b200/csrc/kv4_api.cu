@@ -34,7 +34,7 @@ int check_cache(const llmfa_kv4_cache* c, const llmfa_kv4_seqs* s, bool lengths,
   if ((1 << shift) != c->page_size) return LLMFA_ERR_INVALID_ARGUMENT;
   if (c->group != 32 && c->group != 64 && c->group != 128) return LLMFA_ERR_INVALID_ARGUMENT;
   if (s->batch > 1 && s->table_stride < s->max_pages) return LLMFA_ERR_INVALID_ARGUMENT;
-  if (!aligned(c->pages, 16) || !aligned(c->positions, 4) || !aligned(c->weights, 4) ||
+  if (!aligned(c->pages, 16) || !aligned(c->positions, 16) || !aligned(c->weights, 16) ||
       !aligned(s->page_table, 4) || !aligned(s->lengths, 4))
     return LLMFA_ERR_UNSUPPORTED;
   if (c->num_pages >= (int64_t(1) << 31) || c->heads > 1024 || s->batch > kKv4MaxBatch ||
@@ -187,6 +187,38 @@ int allow_smem(size_t bytes) {
     return LLMFA_ERR_CUDA;
   }
   done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  return LLMFA_OK;
+}
+
+int select_launch(const Kv4SelectParams& p, long long capacity, int sms, int32_t* movers,
+                  cudaStream_t st) {
+  const long long units = static_cast<long long>(p.seqs.batch) * p.pool.heads;
+  const int ctas = kv4_select_ctas(units, capacity, sms);
+  const int run = kv4_select_run(capacity, ctas);
+  const bool in_smem = kv4_select_in_smem(capacity);
+  const size_t smem = sizeof(Kv4SelectSmem) + static_cast<size_t>(run) / 8 +
+                      (in_smem ? static_cast<size_t>(run) * 4 : 0);
+  constexpr size_t kMost = 227 * 1024;
+  if (smem > kMost || units * ctas >= (1ll << 31)) return LLMFA_ERR_UNSUPPORTED;
+  int rc;
+  if ((rc = in_smem ? allow_smem<kv4_select_kernel<true>>(kMost)
+                    : allow_smem<kv4_select_kernel<false>>(kMost)) != LLMFA_OK)
+    return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * ctas));
+  cfg.blockDim = dim3(kKv4SelectThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {static_cast<unsigned>(ctas), 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, in_smem ? kv4_select_kernel<true> : kv4_select_kernel<false>, p, movers,
+                         ctas) != cudaSuccess) {
+    cudaGetLastError();
+    return LLMFA_ERR_LAUNCH;
+  }
   return LLMFA_OK;
 }
 
@@ -368,9 +400,10 @@ int llmfa_kv4_evict_select(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* s
   p.new_lengths = new_lengths;
   p.keep = static_cast<int>(keep);
   p.recent = static_cast<int>(recent);
-  kv4_select_kernel<<<static_cast<unsigned>(seqs->batch * cache->heads), kKv4SelectThreads, 0,
-                      static_cast<cudaStream_t>(stream)>>>(p, static_cast<int32_t*>(workspace));
-  return launched();
+  int sms = 0;
+  if ((rc = device_sms(&sms)) != LLMFA_OK) return rc;
+  return select_launch(p, kv4_capacity(p.pool, p.seqs), sms, static_cast<int32_t*>(workspace),
+                       static_cast<cudaStream_t>(stream));
 }
 
 int llmfa_kv4_evict_move(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs,

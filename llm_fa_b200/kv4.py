@@ -21,26 +21,24 @@ through device_status() (include/llm_fa_b200.h names the codes).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 import math
 
 import torch
 
 from . import _lib
-from .attention import HEAD_DIM
+from .attention import HEAD_DIM, _strides3
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 GROUPS = (32, 64, 128)
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 _DTYPES = {torch.bfloat16: _lib.LLMFA_BF16, torch.float16: _lib.LLMFA_FP16}
 
 
 def page_bytes(page_size: int, group: int) -> int:
     """Bytes of one page of one head."""
-    out = ctypes.c_uint64(0)
-    _lib.check(_lib.lib().llmfa_kv4_page_bytes(int(page_size), int(group), ctypes.byref(out)),
-               "llmfa_kv4_page_bytes")
-    return int(out.value)
+    return _size("llmfa_kv4_page_bytes", int(page_size), int(group))
 
 
 class KV4Cache:
@@ -76,6 +74,8 @@ class KV4Cache:
         # read-only from here on: the C struct holds their addresses
         self._pages, self._positions, self._weights = pages, positions, weights
         self.page_size, self.group = page_size, group
+        self._device, self._index = pages.device, pages.get_device()
+        self._heads = pages.shape[1]
         self._c = _lib.Kv4Cache(pages.data_ptr(), positions.data_ptr(), weights.data_ptr(),
                                 pages.shape[0], pages.shape[1], page_size, group)
 
@@ -105,65 +105,83 @@ class KV4Cache:
 
     @property
     def device(self) -> torch.device:
-        return self._pages.device
+        return self._device
 
     @property
     def heads(self) -> int:
-        return self._pages.shape[1]
+        return self._heads
 
+
+# A step of a small batch costs a few microseconds on the GPU, so the checks below read each
+# property of a tensor once.
 
 def _ints(t: torch.Tensor, name: str, cache: KV4Cache, batch: int) -> int:
-    if t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.dim() != 1 or t.size(0) != batch or not t.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous int32 of shape ({batch},), got {t.dtype} "
                            f"{tuple(t.shape)}")
-    if t.device != cache.device:
-        raise RuntimeError(f"{name} is on {t.device}, expected {cache.device}")
+    if t.get_device() != cache._index:
+        raise RuntimeError(f"{name} is on {t.device}, expected {cache._device}")
     return t.data_ptr()
 
 
 def _seqs(cache: KV4Cache, page_table: torch.Tensor, lengths: torch.Tensor | None) -> _lib.Kv4Seqs:
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or 0 in page_table.shape:
+    shape = page_table.shape
+    if len(shape) != 2 or page_table.dtype != torch.int32 or 0 in shape:
         raise RuntimeError("page_table must be int32 [batch, max_pages], got "
-                           f"{page_table.dtype} {tuple(page_table.shape)}")
-    if page_table.device != cache.device:
-        raise RuntimeError(f"page_table is on {page_table.device}, expected {cache.device}")
-    batch, width = page_table.shape
-    if width > 1 and page_table.stride(1) != 1:
+                           f"{page_table.dtype} {tuple(shape)}")
+    if page_table.get_device() != cache._index:
+        raise RuntimeError(f"page_table is on {page_table.device}, expected {cache._device}")
+    batch, width = shape
+    row, col = page_table.stride()
+    if width > 1 and col != 1:
         raise RuntimeError("page_table rows must be contiguous (stride 1)")
-    if batch > 1 and page_table.stride(0) < width:
+    if batch > 1 and row < width:
         raise RuntimeError("page_table rows must not overlap")
-    return _lib.Kv4Seqs(page_table.data_ptr(), page_table.stride(0), width,
+    return _lib.Kv4Seqs(page_table.data_ptr(), row, width,
                         None if lengths is None else _ints(lengths, "lengths", cache, batch), batch)
 
 
 def _rows(t: torch.Tensor, name: str, cache: KV4Cache, batch: int, heads: int | None,
-          like: torch.Tensor | None = None) -> None:
-    """One [batch, tokens, heads, 128] tensor of 16-bit values."""
-    if t.device != cache.device:
-        raise RuntimeError(f"{name} is on {t.device}, expected {cache.device}")
+          like: torch.Tensor | None = None):
+    """Checks one [batch, tokens, heads, 128] tensor of 16-bit values; (shape, strides)."""
+    shape, stride = t.shape, t.stride()
+    if t.get_device() != cache._index:
+        raise RuntimeError(f"{name} is on {t.device}, expected {cache._device}")
     if t.dtype not in _DTYPES:
         raise RuntimeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
-    if t.dim() != 4 or t.shape[3] != HEAD_DIM or t.shape[0] != batch or (
-            heads is not None and t.shape[2] != heads):
+    if len(shape) != 4 or shape[3] != HEAD_DIM or shape[0] != batch or (
+            heads is not None and shape[2] != heads):
         raise RuntimeError(f"{name} must be [{batch}, tokens, {heads or 'heads'}, {HEAD_DIM}], got "
-                           f"shape {tuple(t.shape)}")
-    if t.shape[1] == 0 or t.shape[2] == 0:
+                           f"shape {tuple(shape)}")
+    if shape[1] == 0 or shape[2] == 0:
         raise RuntimeError(f"empty {name} is not supported")
-    if t.stride(-1) != 1:
+    if stride[3] != 1:
         raise RuntimeError(f"{name} head dim must be contiguous (stride 1)")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype):
+    if like is not None and (shape != like.shape or t.dtype != like.dtype):
         raise RuntimeError(f"{name} must be {like.dtype} {tuple(like.shape)}, got {t.dtype} "
-                           f"{tuple(t.shape)}")
+                           f"{tuple(shape)}")
+    return shape, _strides3(stride)
 
 
-def _on(device: torch.device):
-    # the library launches on the current device: switch only when the tensors live elsewhere
-    return (torch.cuda.device(device) if device.index != torch.cuda.current_device()
-            else contextlib.nullcontext())
+def _call(cache: KV4Cache, name: str, *args) -> None:
+    """One library call on the cache's device and its current stream (the last argument)."""
+    index = cache._index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        rc = getattr(_lib.lib(), name)(cache._c, *args, stream)
+    else:  # the library launches on the current device
+        with torch.cuda.device(index):
+            rc = getattr(_lib.lib(), name)(cache._c, *args, stream)
+    if rc != _lib.LLMFA_OK:
+        _lib.check(rc, name)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+@functools.lru_cache(maxsize=256)
+def _size(name: str, *args: int) -> int:
+    """A workspace size of the library."""
+    out = ctypes.c_uint64(0)
+    _lib.check(getattr(_lib.lib(), name)(*args, ctypes.byref(out)), name)
+    return int(out.value)
 
 
 def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
@@ -176,16 +194,12 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, page_table: to
     differs from lengths once tokens were evicted. lengths itself is not changed.
     """
     seqs = _seqs(cache, page_table, lengths)
-    B = page_table.shape[0]
-    _rows(k, "k", cache, B, cache.heads)
-    _rows(v, "v", cache, B, cache.heads, like=k)
-    with _on(cache.device):
-        _lib.check(_lib.lib().llmfa_kv4_append(
-            cache._c, seqs, k.data_ptr(), _lib.strides3(k.stride()[:3]), v.data_ptr(),
-            _lib.strides3(v.stride()[:3]),
-            None if counts is None else _ints(counts, "counts", cache, B),
-            None if seen is None else _ints(seen, "seen", cache, B), k.shape[1], _DTYPES[k.dtype],
-            _stream(cache.device)), "llmfa_kv4_append")
+    B = seqs.batch
+    shape, ks = _rows(k, "k", cache, B, cache._heads)
+    _, vs = _rows(v, "v", cache, B, cache._heads, like=k)
+    _call(cache, "llmfa_kv4_append", seqs, k.data_ptr(), ks, v.data_ptr(), vs,
+          None if counts is None else _ints(counts, "counts", cache, B),
+          None if seen is None else _ints(seen, "seen", cache, B), shape[1], _DTYPES[k.dtype])
 
 
 def kv4_expand(cache: KV4Cache, page_table: torch.Tensor, start: torch.Tensor, tokens: int, *,
@@ -194,24 +208,21 @@ def kv4_expand(cache: KV4Cache, page_table: torch.Tensor, start: torch.Tensor, t
     """(k, v) [batch, tokens, heads, 128] of slots start[b] .. start[b] + counts[b] - 1 (counts
     default: tokens); rows past a count are zeros. With `out`, fills and returns that pair."""
     seqs = _seqs(cache, page_table, start)
-    B = page_table.shape[0]
+    B = seqs.batch
     if out is None:
         if dtype not in _DTYPES or tokens < 1:
             raise RuntimeError("kv4_expand needs tokens >= 1 and bfloat16 or float16, got "
                                f"{tokens}, {dtype}")
-        out = tuple(torch.empty(B, tokens, cache.heads, HEAD_DIM, dtype=dtype, device=cache.device)
-                    for _ in range(2))
+        shape = (B, tokens, cache._heads, HEAD_DIM)
+        out = (torch.empty(shape, dtype=dtype, device=cache._device),
+               torch.empty(shape, dtype=dtype, device=cache._device))
     k, v = out
-    _rows(k, "k", cache, B, cache.heads)
-    _rows(v, "v", cache, B, cache.heads, like=k)
-    if k.shape[1] != tokens:
-        raise RuntimeError(f"out holds {k.shape[1]} tokens, expected {tokens}")
-    with _on(cache.device):
-        _lib.check(_lib.lib().llmfa_kv4_expand(
-            cache._c, seqs, k.data_ptr(), _lib.strides3(k.stride()[:3]), v.data_ptr(),
-            _lib.strides3(v.stride()[:3]),
-            None if counts is None else _ints(counts, "counts", cache, B), tokens,
-            _DTYPES[k.dtype], _stream(cache.device)), "llmfa_kv4_expand")
+    shape, ks = _rows(k, "k", cache, B, cache._heads)
+    _, vs = _rows(v, "v", cache, B, cache._heads, like=k)
+    if shape[1] != tokens:
+        raise RuntimeError(f"out holds {shape[1]} tokens, expected {tokens}")
+    _call(cache, "llmfa_kv4_expand", seqs, k.data_ptr(), ks, v.data_ptr(), vs,
+          None if counts is None else _ints(counts, "counts", cache, B), tokens, _DTYPES[k.dtype])
     return k, v
 
 
@@ -236,34 +247,32 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
     log-sum-exp of every row, fp32 [batch, heads_q, tokens].
     """
     seqs = _seqs(cache, page_table, lengths)
-    B = page_table.shape[0]
-    _rows(q, "q", cache, B, None)
-    T, Hq = q.shape[1], q.shape[2]
-    if Hq % cache.heads != 0:
-        raise RuntimeError(f"q has {Hq} heads, not a multiple of the cache's {cache.heads}")
-    if decay is not None and not 0.0 <= decay <= 1.0:
+    B = seqs.batch
+    shape, qs = _rows(q, "q", cache, B, None)
+    T, Hq = shape[1], shape[2]
+    if Hq % cache._heads != 0:
+        raise RuntimeError(f"q has {Hq} heads, not a multiple of the cache's {cache._heads}")
+    if decay is None:
+        decay = -1.0
+    elif not 0.0 <= decay <= 1.0:
         raise RuntimeError(f"decay must be between 0 and 1, got {decay}")
     n = None if counts is None else _ints(counts, "counts", cache, B)
     if out is None:
-        out = (torch.empty if counts is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+        out = (torch.empty if counts is None else torch.zeros)(shape, dtype=q.dtype,
+                                                               device=cache._device)
+        os = _strides3(out.stride())
     else:
-        _rows(out, "out", cache, B, Hq, like=q)
-    scale = (1.0 / math.sqrt(HEAD_DIM)) if softmax_scale is None else float(softmax_scale)
-    lib = _lib.lib()
-    need = ctypes.c_uint64(0)
-    with _on(cache.device):
-        _lib.check(lib.llmfa_kv4_attention_workspace_size(B, cache.heads, Hq, T, ctypes.byref(need)),
-                   "llmfa_kv4_attention_workspace_size")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=cache.device)
-        lse = None
-        if return_lse:
-            lse = torch.full((B, Hq, T), -math.inf, dtype=torch.float32, device=cache.device)
-        _lib.check(lib.llmfa_kv4_attention(
-            cache._c, seqs, q.data_ptr(), _lib.strides3(q.stride()[:3]), out.data_ptr(),
-            _lib.strides3(out.stride()[:3]), lse.data_ptr() if return_lse else None,
-            _lib.strides2((Hq * T, T)), n, Hq, T, int(causal), scale,
-            -1.0 if decay is None else float(decay), _DTYPES[q.dtype], ws.data_ptr(), need.value,
-            _stream(cache.device)), "llmfa_kv4_attention")
+        _, os = _rows(out, "out", cache, B, Hq, like=q)
+    nbytes = _size("llmfa_kv4_attention_workspace_size", B, cache._heads, Hq, T)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache._device)
+    lse = ls = None
+    if return_lse:
+        lse = torch.full((B, Hq, T), -math.inf, dtype=torch.float32, device=cache._device)
+        ls = _lib.strides2((Hq * T, T))
+    _call(cache, "llmfa_kv4_attention", seqs, q.data_ptr(), qs, out.data_ptr(), os,
+          lse.data_ptr() if return_lse else None, ls, n, Hq, T, bool(causal),
+          _SCALE if softmax_scale is None else softmax_scale, decay, _DTYPES[q.dtype],
+          ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -278,35 +287,28 @@ def kv4_evict_select(cache: KV4Cache, page_table: torch.Tensor, lengths: torch.T
     past the new length; freed slots take the survivors from above `keep` in order.
     """
     seqs = _seqs(cache, page_table, lengths)
-    B = page_table.shape[0]
+    B = seqs.batch
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise RuntimeError(f"keep must be at least 1 and recent 0 to keep, got {keep}, {recent}")
-    s = None if seen is None else _ints(seen, "seen", cache, B)
-    lib = _lib.lib()
-    need = ctypes.c_uint64(0)
-    with _on(cache.device):
-        src = torch.empty(B, cache.heads, keep, dtype=torch.int32, device=cache.device)
-        new = torch.empty(B, dtype=torch.int32, device=cache.device)
-        _lib.check(lib.llmfa_kv4_evict_workspace_size(B, cache.heads, keep, ctypes.byref(need)),
-                   "llmfa_kv4_evict_workspace_size")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=cache.device)
-        _lib.check(lib.llmfa_kv4_evict_select(
-            cache._c, seqs, s, keep, recent, src.data_ptr(), new.data_ptr(), ws.data_ptr(),
-            need.value, _stream(cache.device)), "llmfa_kv4_evict_select")
+    src = torch.empty((B, cache._heads, keep), dtype=torch.int32, device=cache._device)
+    new = torch.empty(B, dtype=torch.int32, device=cache._device)
+    nbytes = _size("llmfa_kv4_evict_workspace_size", B, cache._heads, keep)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=cache._device)
+    _call(cache, "llmfa_kv4_evict_select", seqs,
+          None if seen is None else _ints(seen, "seen", cache, B), keep, recent, src.data_ptr(),
+          new.data_ptr(), ws.data_ptr(), nbytes)
     return src, new
 
 
 def kv4_evict_move(cache: KV4Cache, page_table: torch.Tensor, src: torch.Tensor) -> None:
     """Make the moves that kv4_evict_select chose (codes, scales, positions and weights)."""
     seqs = _seqs(cache, page_table, None)
-    want = (page_table.shape[0], cache.heads)
-    if src.dim() != 3 or src.shape[:2] != want or src.dtype != torch.int32 or src.shape[2] == 0 \
-            or not src.is_contiguous():
-        raise RuntimeError(f"src must be contiguous int32 [{want[0]}, {want[1]}, keep], got "
-                           f"{src.dtype} {tuple(src.shape)}")
-    if src.device != cache.device:
-        raise RuntimeError(f"src is on {src.device}, expected {cache.device}")
-    with _on(cache.device):
-        _lib.check(_lib.lib().llmfa_kv4_evict_move(cache._c, seqs, src.data_ptr(), src.shape[2],
-                                                   _stream(cache.device)), "llmfa_kv4_evict_move")
+    shape = src.shape
+    if len(shape) != 3 or shape[0] != seqs.batch or shape[1] != cache._heads or shape[2] == 0 \
+            or src.dtype != torch.int32 or not src.is_contiguous():
+        raise RuntimeError(f"src must be contiguous int32 [{seqs.batch}, {cache._heads}, keep], got "
+                           f"{src.dtype} {tuple(shape)}")
+    if src.get_device() != cache._index:
+        raise RuntimeError(f"src is on {src.device}, expected {cache._device}")
+    _call(cache, "llmfa_kv4_evict_move", seqs, src.data_ptr(), shape[2])

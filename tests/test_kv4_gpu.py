@@ -446,7 +446,7 @@ def check_select(cache, table, lens, keep, recent, seen):
 @pytest.mark.parametrize("lens,keep,recent,page,H", [
     ([1], 1, 0, 16, 1), ([2], 1, 1, 16, 2), ([17, 16, 0], 16, 3, 16, 3), ([700, 3, 40], 33, 33, 64, 2),
     ([2049], 2048, 64, 64, 2), ([5000, 4096], 1500, 100, 256, 1), ([300], 299, 0, 32, 4),
-    ([100], 300, 5, 128, 1),
+    ([100], 300, 5, 128, 1), ([40001, 33000], 20000, 500, 64, 1),
 ])
 def test_select(kind, lens, keep, recent, page, H):
     cache, table = pool(len(lens), H, max(lens), page, 64, seed=1)
@@ -455,6 +455,17 @@ def test_select(kind, lens, keep, recent, page, H):
     cache.positions.copy_(torch.randint(0, 2 * max(lens), cache.positions.shape, generator=gen))
     check_select(cache, table, lens, keep, recent, None)
     check_select(cache, table, lens, keep, recent, [2 * n for n in lens])
+    assert device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["spread", "ties", "special"])
+def test_select_from_a_table_too_long_for_shared_memory(kind):
+    """A page table of 409,600 slots, of which 9000 are used."""
+    cache, table = pool(1, 2, 9000, 256, 64, seed=2)
+    weights_like(cache, kind, seed=7)
+    wide = torch.full((1, 1600), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    check_select(cache, wide, [9000], 3000, 100, None)
     assert device_status() == 0
 
 
