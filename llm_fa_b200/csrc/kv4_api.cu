@@ -82,8 +82,13 @@ int by_type_and_groups(int dtype, int ng, F f) {
   return dtype == LLMFA_BF16 ? groups(__nv_bfloat16{}) : groups(__half{});
 }
 
-int64_t quant_blocks(int64_t rows) {
-  return (rows * kKv4RowThreads + kKv4QuantThreads - 1) / kKv4QuantThreads;
+// Grid of append and expand: a token's heads in x, sequences in y.
+int quant_grid(int64_t batch, int64_t tokens, int64_t heads, dim3* grid) {
+  if (tokens * heads >= (int64_t(1) << 31) / kKv4RowThreads) return LLMFA_ERR_UNSUPPORTED;
+  *grid = dim3(static_cast<unsigned>((tokens * heads * kKv4RowThreads + kKv4QuantThreads - 1) /
+                                     kKv4QuantThreads),
+               static_cast<unsigned>(batch));
+  return LLMFA_OK;
 }
 
 // Rows of a key head, cut into tiles of 8 nt: the fewest tiles, then the least padding.
@@ -270,15 +275,16 @@ int llmfa_kv4_append(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, c
   if ((rc = check_rows(k, k_strides, seqs->batch, tokens, cache->heads, &p.k)) != LLMFA_OK) return rc;
   if ((rc = check_rows(v, v_strides, seqs->batch, tokens, cache->heads, &p.v)) != LLMFA_OK) return rc;
   if (!aligned(seen, 4)) return LLMFA_ERR_UNSUPPORTED;
-  const int64_t blocks = quant_blocks(seqs->batch * tokens * cache->heads);
-  if (blocks >= (int64_t(1) << 31)) return LLMFA_ERR_UNSUPPORTED;
+  dim3 grid;
+  if ((rc = quant_grid(seqs->batch, tokens, cache->heads, &grid)) != LLMFA_OK) return rc;
   if ((rc = device_status_ptr(&p.seqs.status)) != LLMFA_OK) return rc;
   p.counts = counts;
   p.seen = seen;
   p.tokens = static_cast<int>(tokens);
+  p.heads = Kv4Div(static_cast<uint32_t>(cache->heads));
   return by_type_and_groups(dtype, p.pool.ng, [&](auto t, auto ng) {
     kv4_append_kernel<decltype(t), ng.value>
-        <<<static_cast<unsigned>(blocks), kKv4QuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        <<<grid, kKv4QuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
     return launched();
   });
 }
@@ -292,14 +298,15 @@ int llmfa_kv4_expand(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, v
   if ((rc = check_tokens(tokens, dtype, counts)) != LLMFA_OK) return rc;
   if ((rc = check_rows(k, k_strides, seqs->batch, tokens, cache->heads, &p.k)) != LLMFA_OK) return rc;
   if ((rc = check_rows(v, v_strides, seqs->batch, tokens, cache->heads, &p.v)) != LLMFA_OK) return rc;
-  const int64_t blocks = quant_blocks(seqs->batch * tokens * cache->heads);
-  if (blocks >= (int64_t(1) << 31)) return LLMFA_ERR_UNSUPPORTED;
+  dim3 grid;
+  if ((rc = quant_grid(seqs->batch, tokens, cache->heads, &grid)) != LLMFA_OK) return rc;
   if ((rc = device_status_ptr(&p.seqs.status)) != LLMFA_OK) return rc;
   p.counts = counts;
   p.tokens = static_cast<int>(tokens);
+  p.heads = Kv4Div(static_cast<uint32_t>(cache->heads));
   return by_type_and_groups(dtype, p.pool.ng, [&](auto t, auto ng) {
     kv4_expand_kernel<decltype(t), ng.value>
-        <<<static_cast<unsigned>(blocks), kKv4QuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        <<<grid, kKv4QuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
     return launched();
   });
 }

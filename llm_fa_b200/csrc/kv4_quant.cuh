@@ -12,11 +12,15 @@
 // kernel takes x * (1 / scale), within 2^-19 of the quotient for |x / scale|
 // <= 16, and adds 768 in one fused step, which rounds to a multiple of 2^-14:
 // half-integers come back exactly, nothing else can reach one, and no divide
-// is needed per value.
+// is needed per value. Adding 1.5 * 2^23 - 768 then rounds to an integer,
+// halves to even, in the low bits. As rounding is monotone and odd, no code
+// falls below 0; only the upper end has to be clamped.
 //
 // Both kernels move bytes: 512 of a token's head on one side, 136 to 160 of
 // codes and pairs on the other. A thread takes 8 channels (one 16-byte access)
-// of the key and the value, 16 threads a token's head.
+// of the key and the value, 16 threads a token's head. What would bound them
+// otherwise is instructions, so ranges are taken on packed pairs, and codes
+// become numbers as fp16 integers.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -33,6 +37,21 @@ struct Kv4RowView {  // [batch, tokens, heads, 128], element strides
   long long sb, st, sh;
 };
 
+// Division of numbers below 2^31 by a d fixed before the launch.
+struct Kv4Div {
+  uint32_t mul, shift, d;
+  Kv4Div() = default;
+  __host__ __device__ explicit Kv4Div(uint32_t by) : mul(0), shift(0), d(by) {
+    while ((uint64_t(1) << shift) < by) ++shift;
+    mul = static_cast<uint32_t>((((uint64_t(1) << shift) - by) << 32) / by + 1);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    return (__umulhi(n, mul) + n) >> shift;
+  }
+#endif
+};
+
 template <typename T>
 struct Kv4Type;
 template <>
@@ -44,6 +63,11 @@ struct Kv4Type<__nv_bfloat16> {
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&h);
   }
+  static __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {  // NaN if either is
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
 };
 template <>
 struct Kv4Type<__half> {
@@ -54,61 +78,70 @@ struct Kv4Type<__half> {
     __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&h);
   }
+  static __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
 };
+
+__device__ __forceinline__ float2 kv4_scale_zero(uint32_t pair) {
+  return make_float2(__uint_as_float(pair << 16), __uint_as_float(pair & 0xffff0000u));
+}
 
 // Scale, its reciprocal and zero of a group from its lo and hi.
 struct Kv4Pair {
-  float scale, inv, zero;
+  float inv;
+  int zero;
   uint32_t word;
 };
-__device__ __forceinline__ float kv4_snap(float x, float inv) {
-  return __fadd_rn(__fmaf_rn(x, inv, 768.f), -768.f);
-}
 __device__ __forceinline__ Kv4Pair kv4_pair(float lo, float hi) {
   Kv4Pair p;
   float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)));
-  // lo and hi skip NaN only in part (see kv4_range): any NaN or infinity shows in hi - lo
+  // a NaN or an infinity in the group shows in hi - lo
   if (!(s < __int_as_float(0x7f800000))) s = __int_as_float(0x7fc00000);
   // Below 2^-120 the reciprocal nears the end of fp32's range: such a group counts as zeros.
   if (s < 0x1p-120f) s = 0.f;
-  p.scale = s;
   p.inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
-  p.zero = fminf(fmaxf(rintf(kv4_snap(-lo, p.inv)), 0.f), 15.f);
-  p.word = (__float_as_uint(s) >> 16) | (__float_as_uint(p.zero) & 0xffff0000u);
+  const float r = __fadd_rn(__fmaf_rn(-lo, p.inv, 768.f), 12582912.f - 768.f);
+  p.zero = min(max(__float_as_int(r) - 0x4B400000, 0), 15);
+  p.word = (__float_as_uint(s) >> 16) | (__float_as_uint(static_cast<float>(p.zero)) & 0xffff0000u);
   return p;
 }
 // 8 values -> 8 codes, low bits first.
-__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], const Kv4Pair& p) {
+template <typename T>
+__device__ __forceinline__ uint32_t kv4_codes(const uint4& raw, const Kv4Pair& p) {
+  const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
+  const int base = p.zero - 0x4B400000;
   uint32_t w = 0;
-  const int zero = static_cast<int>(p.zero);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // round to an integer by adding 1.5 * 2^23: halves to even, before zero is added
-    const int r = __float_as_int(__fadd_rn(kv4_snap(x[i], p.inv), 12582912.f)) - 0x4B400000;
-    const int u = min(max(r + zero, 0), 15);
-    w |= static_cast<uint32_t>(u) << (4 * i);
+  for (int i = 3; i >= 0; --i) {
+    const float2 x = Kv4Type<T>::unpack(r[i]);
+#pragma unroll
+    for (int k = 1; k >= 0; --k) {
+      const float v = __fadd_rn(__fmaf_rn(k ? x.y : x.x, p.inv, 768.f), 12582912.f - 768.f);
+      w = w * 16 + min(__float_as_int(v) + base, 15);
+    }
   }
   return w;
 }
-// lo and hi of a group over the 16 / NG threads that hold it; NaN reaches both.
-template <int NG>
-__device__ __forceinline__ void kv4_range(const float (&x)[8], float& lo, float& hi) {
-  lo = 0.f;
-  hi = 0.f;
-  float bad = 0.f;
+// lo = min(0, x) and hi = max(0, x) of a group, over the 16 / NG threads that hold it; a NaN in it
+// makes one of them NaN. Both are minima: of x, and of -x with its sign bits flipped.
+template <typename T, int NG>
+__device__ __forceinline__ float2 kv4_range(const uint4& raw) {
+  constexpr uint32_t kSigns = 0x80008000u;
+  using V = Kv4Type<T>;
+  const uint32_t lo2 = V::min2(V::min2(raw.x, raw.y), V::min2(raw.z, raw.w));
+  const uint32_t hi2 = V::min2(V::min2(raw.x ^ kSigns, raw.y ^ kSigns),
+                               V::min2(raw.z ^ kSigns, raw.w ^ kSigns));
+  // (lo, -hi) of the thread, then of the group
+  uint32_t both = V::min2(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));
+  both = V::min2(both, 0u);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad += x[i] * 0.f;  // NaN for NaN and infinities
-  }
-  hi += bad;
-#pragma unroll
-  for (int d = 1; d < kKv4RowThreads / NG; d <<= 1) {
-    const float l = __shfl_xor_sync(0xffffffffu, lo, d), h = __shfl_xor_sync(0xffffffffu, hi, d);
-    lo = fminf(lo, l);
-    hi = h != h ? h : hi != hi ? hi : fmaxf(hi, h);
-  }
+  for (int d = 1; d < kKv4RowThreads / NG; d <<= 1)
+    both = V::min2(both, __shfl_xor_sync(0xffffffffu, both, d));
+  const float2 f = V::unpack(both);
+  return make_float2(f.x, -f.y);
 }
 
 struct Kv4AppendParams {
@@ -118,52 +151,48 @@ struct Kv4AppendParams {
   const int32_t* counts;  // new tokens of a sequence, or null
   const int32_t* seen;    // position of its first new token, or null: its length
   int tokens;
+  Kv4Div heads;
 };
 
-// One 16-thread row a (sequence, token, head); heads run fastest, as in memory.
+// A thread's row: 16 threads a (token, head) of sequence blockIdx.y; heads run fastest, as in
+// memory.
+struct Kv4QuantRow {
+  int b, t, h;
+  bool live;
+};
+__device__ __forceinline__ Kv4QuantRow kv4_quant_row(const Kv4Div& heads, int tokens) {
+  const uint32_t row = (blockIdx.x * kKv4QuantThreads + threadIdx.x) / kKv4RowThreads;
+  const uint32_t t = heads.quotient(row);
+  return {static_cast<int>(blockIdx.y), static_cast<int>(t), static_cast<int>(row - t * heads.d),
+          t < static_cast<uint32_t>(tokens)};
+}
+
 template <typename T, int NG>
-__global__ void __launch_bounds__(kKv4QuantThreads) kv4_append_kernel(Kv4AppendParams p) {
-  const long long row = (static_cast<long long>(blockIdx.x) * kKv4QuantThreads + threadIdx.x) /
-                        kKv4RowThreads;
+__global__ void __launch_bounds__(kKv4QuantThreads)
+    kv4_append_kernel(const __grid_constant__ Kv4AppendParams p) {
+  const Kv4QuantRow row = kv4_quant_row(p.heads, p.tokens);
   const int w = threadIdx.x % kKv4RowThreads;  // natural word: channels 8w .. 8w + 7
-  const int heads = p.pool.heads;
-  const long long rows = static_cast<long long>(p.seqs.batch) * p.tokens * heads;
-  bool live = row < rows;
-  const int h = live ? static_cast<int>(row % heads) : 0;
-  const long long bt = live ? row / heads : 0;
-  const int t = static_cast<int>(bt % p.tokens), b = static_cast<int>(bt / p.tokens);
-  long long page = -1, slot = 0;
-  if (live) {
-    live = t < kv4_count(p.seqs, p.counts, b, p.tokens);
-    slot = static_cast<long long>(p.seqs.lengths[b]) + t;
-    if (live) {
-      page = kv4_page(p.pool, p.seqs, b, slot);
-      if (page < 0) kv4_report(p.seqs, kStatusKv4BadPage);
-      live = page >= 0;
-    }
-  }
+  const int b = row.b, t = row.t, h = row.h;
+  const int held = p.seqs.lengths[b];
+  const long long slot = static_cast<long long>(held) + t;
+  bool live = row.live && t < kv4_count(p.seqs, p.counts, b, p.tokens);
+  long long page = -1;
   uint4 raw[2] = {};
   if (live) {
-    const long long at[2] = {b * p.k.sb + t * p.k.st + h * p.k.sh,
-                             b * p.v.sb + t * p.v.st + h * p.v.sh};
-    raw[0] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.k.ptr) + at[0] + 8 * w);
-    raw[1] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v.ptr) + at[1] + 8 * w);
+    page = kv4_page(p.pool, p.seqs, b, slot);
+    raw[0] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.k.ptr) + b * p.k.sb + t * p.k.st +
+                                             h * p.k.sh + 8 * w);
+    raw[1] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v.ptr) + b * p.v.sb + t * p.v.st +
+                                             h * p.v.sh + 8 * w);
+    if (page < 0) kv4_report(p.seqs, kStatusKv4BadPage);
+    live = page >= 0;
   }
   uint32_t code[2], pair[2];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
-    float x[8];
-    const uint32_t* r = reinterpret_cast<const uint32_t*>(&raw[side]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Kv4Type<T>::unpack(r[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-    float lo, hi;
-    kv4_range<NG>(x, lo, hi);
-    const Kv4Pair q = kv4_pair(lo, hi);
-    code[side] = kv4_codes(x, q);
+    const float2 range = kv4_range<T, NG>(raw[side]);
+    const Kv4Pair q = kv4_pair(range.x, range.y);
+    code[side] = kv4_codes<T>(raw[side], q);
     pair[side] = q.word;
   }
   // Values are stored by half-words: natural half-words 2w and 2w + 1 are k = w / 4, g = 2 (w % 4)
@@ -188,7 +217,7 @@ __global__ void __launch_bounds__(kKv4QuantThreads) kv4_append_kernel(Kv4AppendP
   }
   if (w == 0) {
     const long long i = kv4_token_index(p.pool, page, h, slot);
-    p.pool.positions[i] = (p.seen != nullptr ? p.seen[b] : p.seqs.lengths[b]) + t;
+    p.pool.positions[i] = (p.seen != nullptr ? p.seen[b] : held) + t;
     p.pool.weights[i] = 0.f;
   }
 }
@@ -199,33 +228,40 @@ struct Kv4ExpandParams {
   Kv4RowView k, v;
   const int32_t* counts;
   int tokens;
+  Kv4Div heads;
 };
 
-__device__ __forceinline__ float2 kv4_scale_zero(uint32_t pair) {
-  return make_float2(__uint_as_float(pair << 16), __uint_as_float(pair & 0xffff0000u));
-}
+// 8 codes as fp16 integers less their zero (0x6400 + u is 1024 + u, and 1024 + 16 u in the next
+// nibble), then fp32 times the scale: exact up to the one rounding to T.
 template <typename T>
 __device__ __forceinline__ uint4 kv4_decode8(uint32_t codes, uint32_t pair) {
   const float2 sz = kv4_scale_zero(pair);
-  uint32_t o[4];
+  const __half2 zero = __float2half2_rn(1024.f + sz.y);
+  const __half2 zero16 = __float2half2_rn(-64.f - sz.y);
+  const __half2 sixteenth = __float2half2_rn(0.0625f);
+  float x[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    o[i] = Kv4Type<T>::pack(sz.x * (static_cast<float>((codes >> (8 * i)) & 15u) - sz.y),
-                            sz.x * (static_cast<float>((codes >> (8 * i + 4)) & 15u) - sz.y));
-  return make_uint4(o[0], o[1], o[2], o[3]);
+  for (int i = 0; i < 4; ++i) {  // nibbles i and i + 4
+    const uint32_t c = i < 2 ? codes : codes >> 8;
+    uint32_t bits;
+    if (i % 2 == 0) asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(bits) : "r"(c));
+    else asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(bits) : "r"(c));
+    const __half2 u = *reinterpret_cast<__half2*>(&bits);
+    const float2 f = __half22float2(i % 2 == 0 ? __hsub2(u, zero) : __hfma2(u, sixteenth, zero16));
+    x[i] = f.x * sz.x;
+    x[i + 4] = f.y * sz.x;
+  }
+  return make_uint4(Kv4Type<T>::pack(x[0], x[1]), Kv4Type<T>::pack(x[2], x[3]),
+                    Kv4Type<T>::pack(x[4], x[5]), Kv4Type<T>::pack(x[6], x[7]));
 }
 
 // The inverse of kv4_append_kernel; rows past a sequence's count are zeros.
 template <typename T, int NG>
-__global__ void __launch_bounds__(kKv4QuantThreads) kv4_expand_kernel(Kv4ExpandParams p) {
-  const long long row = (static_cast<long long>(blockIdx.x) * kKv4QuantThreads + threadIdx.x) /
-                        kKv4RowThreads;
-  const int w = threadIdx.x % kKv4RowThreads;
-  const int heads = p.pool.heads;
-  if (row >= static_cast<long long>(p.seqs.batch) * p.tokens * heads) return;
-  const int h = static_cast<int>(row % heads);
-  const long long bt = row / heads;
-  const int t = static_cast<int>(bt % p.tokens), b = static_cast<int>(bt / p.tokens);
+__global__ void __launch_bounds__(kKv4QuantThreads)
+    kv4_expand_kernel(const __grid_constant__ Kv4ExpandParams p) {
+  const Kv4QuantRow row = kv4_quant_row(p.heads, p.tokens);
+  if (!row.live) return;
+  const int w = threadIdx.x % kKv4RowThreads, b = row.b, t = row.t, h = row.h;
   uint4 k = make_uint4(0, 0, 0, 0), v = k;
   if (t < kv4_count(p.seqs, p.counts, b, p.tokens)) {
     const long long slot = static_cast<long long>(p.seqs.lengths[b]) + t;
