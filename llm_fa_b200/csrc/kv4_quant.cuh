@@ -17,10 +17,10 @@
 // falls below 0; only the upper end has to be clamped.
 //
 // Both kernels move bytes: 512 of a token's head on one side, 136 to 160 of
-// codes and pairs on the other. A thread takes 8 channels (one 16-byte access)
-// of the key and the value, 16 threads a token's head. What would bound them
-// otherwise is instructions, so ranges are taken on packed pairs, and codes
-// become numbers as fp16 integers.
+// codes and pairs on the other. What would bound them otherwise is
+// instructions: a thread takes 16 channels of the key and the value, so that
+// the addresses of a token's head are worked out by 8 threads; ranges are taken
+// on packed pairs; codes become numbers as fp16 integers.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,7 +30,7 @@
 namespace llmfa {
 
 constexpr int kKv4QuantThreads = 256;
-constexpr int kKv4RowThreads = 16;  // threads of a token's head
+constexpr int kKv4RowThreads = 8;  // threads of a token's head, 16 channels each
 
 struct Kv4RowView {  // [batch, tokens, heads, 128], element strides
   void* ptr;
@@ -95,17 +95,28 @@ struct Kv4Pair {
   int zero;
   uint32_t word;
 };
+// x / 15, correctly rounded: the product with 1/15 and one correction by its exact remainder
+// (Markstein's scheme; compared with the quotient for every mantissa).
+__device__ __forceinline__ float kv4_fifteenth(float x) {
+  constexpr float c = 1.f / 15.f;
+  const float q = __fmul_rn(x, c);
+  return __fmaf_rn(__fmaf_rn(-15.f, q, x), c, q);
+}
 __device__ __forceinline__ Kv4Pair kv4_pair(float lo, float hi) {
   Kv4Pair p;
-  float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)));
+  const float span = __fsub_rn(hi, lo);
+  float s = __bfloat162float(__float2bfloat16_rn(kv4_fifteenth(span)));
   // a NaN or an infinity in the group shows in hi - lo
-  if (!(s < __int_as_float(0x7f800000))) s = __int_as_float(0x7fc00000);
+  if (!(span < __int_as_float(0x7f800000))) s = __int_as_float(0x7fc00000);
   // Below 2^-120 the reciprocal nears the end of fp32's range: such a group counts as zeros.
   if (s < 0x1p-120f) s = 0.f;
-  p.inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  p.inv = s > 0.f ? inv : 0.f;
   const float r = __fadd_rn(__fmaf_rn(-lo, p.inv, 768.f), 12582912.f - 768.f);
-  p.zero = min(max(__float_as_int(r) - 0x4B400000, 0), 15);
-  p.word = (__float_as_uint(s) >> 16) | (__float_as_uint(static_cast<float>(p.zero)) & 0xffff0000u);
+  const float zero = fminf(fmaxf(__fadd_rn(r, -12582912.f), 0.f), 15.f);
+  p.zero = __float_as_int(__fadd_rn(zero, 12582912.f)) - 0x4B400000;
+  p.word = __byte_perm(__float_as_uint(s), __float_as_uint(zero), 0x7632);
   return p;
 }
 // 8 values -> 8 codes, low bits first.
@@ -125,18 +136,21 @@ __device__ __forceinline__ uint32_t kv4_codes(const uint4& raw, const Kv4Pair& p
   }
   return w;
 }
-// lo = min(0, x) and hi = max(0, x) of a group, over the 16 / NG threads that hold it; a NaN in it
+// lo = min(0, x) and hi = max(0, x) of a group, over the 8 / NG threads that hold it; a NaN in it
 // makes one of them NaN. Both are minima: of x, and of -x with its sign bits flipped.
 template <typename T, int NG>
-__device__ __forceinline__ float2 kv4_range(const uint4& raw) {
+__device__ __forceinline__ float2 kv4_range(const uint4 (&raw)[2]) {
   constexpr uint32_t kSigns = 0x80008000u;
   using V = Kv4Type<T>;
-  const uint32_t lo2 = V::min2(V::min2(raw.x, raw.y), V::min2(raw.z, raw.w));
-  const uint32_t hi2 = V::min2(V::min2(raw.x ^ kSigns, raw.y ^ kSigns),
-                               V::min2(raw.z ^ kSigns, raw.w ^ kSigns));
-  // (lo, -hi) of the thread, then of the group
-  uint32_t both = V::min2(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));
-  both = V::min2(both, 0u);
+  uint32_t both = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t lo2 = V::min2(V::min2(raw[i].x, raw[i].y), V::min2(raw[i].z, raw[i].w));
+    const uint32_t hi2 = V::min2(V::min2(raw[i].x ^ kSigns, raw[i].y ^ kSigns),
+                                 V::min2(raw[i].z ^ kSigns, raw[i].w ^ kSigns));
+    // (lo, -hi) of the thread, then of the group
+    both = V::min2(both, V::min2(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632)));
+  }
 #pragma unroll
   for (int d = 1; d < kKv4RowThreads / NG; d <<= 1)
     both = V::min2(both, __shfl_xor_sync(0xffffffffu, both, d));
@@ -154,7 +168,7 @@ struct Kv4AppendParams {
   Kv4Div heads;
 };
 
-// A thread's row: 16 threads a (token, head) of sequence blockIdx.y; heads run fastest, as in
+// A thread's row: 8 threads a (token, head) of sequence blockIdx.y; heads run fastest, as in
 // memory.
 struct Kv4QuantRow {
   int b, t, h;
@@ -171,51 +185,60 @@ template <typename T, int NG>
 __global__ void __launch_bounds__(kKv4QuantThreads)
     kv4_append_kernel(const __grid_constant__ Kv4AppendParams p) {
   const Kv4QuantRow row = kv4_quant_row(p.heads, p.tokens);
-  const int w = threadIdx.x % kKv4RowThreads;  // natural word: channels 8w .. 8w + 7
+  const int a = threadIdx.x % kKv4RowThreads;  // channels 16a .. 16a + 15: natural words 2a, 2a + 1
   const int b = row.b, t = row.t, h = row.h;
   const int held = p.seqs.lengths[b];
   const long long slot = static_cast<long long>(held) + t;
   bool live = row.live && t < kv4_count(p.seqs, p.counts, b, p.tokens);
   long long page = -1;
-  uint4 raw[2] = {};
+  uint4 raw[2][2] = {};
   if (live) {
     page = kv4_page(p.pool, p.seqs, b, slot);
-    raw[0] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.k.ptr) + b * p.k.sb + t * p.k.st +
-                                             h * p.k.sh + 8 * w);
-    raw[1] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v.ptr) + b * p.v.sb + t * p.v.st +
-                                             h * p.v.sh + 8 * w);
+    const uint4* k = reinterpret_cast<const uint4*>(static_cast<const T*>(p.k.ptr) + b * p.k.sb +
+                                                    t * p.k.st + h * p.k.sh + 16 * a);
+    const uint4* v = reinterpret_cast<const uint4*>(static_cast<const T*>(p.v.ptr) + b * p.v.sb +
+                                                    t * p.v.st + h * p.v.sh + 16 * a);
+    raw[0][0] = k[0];
+    raw[0][1] = k[1];
+    raw[1][0] = v[0];
+    raw[1][1] = v[1];
     if (page < 0) kv4_report(p.seqs, kStatusKv4BadPage);
     live = page >= 0;
   }
-  uint32_t code[2], pair[2];
+  uint32_t code[2][2], pair[2];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const float2 range = kv4_range<T, NG>(raw[side]);
     const Kv4Pair q = kv4_pair(range.x, range.y);
-    code[side] = kv4_codes<T>(raw[side], q);
+    code[side][0] = kv4_codes<T>(raw[side][0], q);
+    code[side][1] = kv4_codes<T>(raw[side][1], q);
     pair[side] = q.word;
   }
-  // Values are stored by half-words: natural half-words 2w and 2w + 1 are k = w / 4, g = 2 (w % 4)
-  // and g + 1. Threads w and w ^ 4 (k and k ^ 1) trade halves, so that each writes one word.
-  const bool odd = (w & 4) != 0;
-  const uint32_t give = odd ? code[1] & 0xffffu : code[1] >> 16;
-  const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 4);
-  const uint32_t vword = odd ? (got | (code[1] & 0xffff0000u)) : ((code[1] & 0xffffu) | (got << 16));
+  // Values are stored by half-words: this thread's are k = a / 2 and g = 4 (a % 2) .. + 3 of the
+  // natural k * 8 + g. Threads a and a ^ 2 (k and k ^ 1) trade halves, so that each writes two
+  // whole words, of the g of its own word (a & 2) / 2.
+  const bool odd = (a & 2) != 0;
+  const uint32_t got = __shfl_xor_sync(0xffffffffu, code[1][odd ? 0 : 1], 2);
+  const uint32_t mine = code[1][odd ? 1 : 0];
+  const uint32_t even_k = odd ? got : mine, odd_k = odd ? mine : got;
   if (!live) return;
   uint8_t* block = p.pool.pages + kv4_block_offset(p.pool, page, h, slot);
   const int tok = static_cast<int>(slot & 15);
   uint8_t* vblock = block + kv4_half_bytes(NG);
-  reinterpret_cast<uint32_t*>(block + tok * kKv4RowBytes)[kv4_key_word(w)] = code[0];
-  // even k: g = 2 (w % 4), halves k, k + 1; odd k: g + 1, halves k - 1, k
-  const int g = 2 * (w & 3) + (odd ? 1 : 0), k = (w >> 2) & ~1;
-  reinterpret_cast<uint32_t*>(vblock + tok * kKv4RowBytes)[g * 2 + k / 2] = vword;
+  uint32_t* krow = reinterpret_cast<uint32_t*>(block + tok * kKv4RowBytes);
+  krow[kv4_key_word(2 * a)] = code[0][0];
+  krow[kv4_key_word(2 * a + 1)] = code[0][1];
+  uint32_t* vrow = reinterpret_cast<uint32_t*>(vblock + tok * kKv4RowBytes);
+  const int g = 4 * (a & 1) + (odd ? 2 : 0), word = g * 2 + (a >> 2);
+  vrow[word] = __byte_perm(even_k, odd_k, 0x5410);
+  vrow[word + 2] = __byte_perm(even_k, odd_k, 0x7632);
   constexpr int kGroupThreads = kKv4RowThreads / NG;
-  if (w % kGroupThreads == 0) {
-    const int at = tok * NG + w / kGroupThreads;
+  if (a % kGroupThreads == 0) {
+    const int at = tok * NG + a / kGroupThreads;
     reinterpret_cast<uint32_t*>(block + kKv4Block * kKv4RowBytes)[at] = pair[0];
     reinterpret_cast<uint32_t*>(vblock + kKv4Block * kKv4RowBytes)[at] = pair[1];
   }
-  if (w == 0) {
+  if (a == 0) {
     const long long i = kv4_token_index(p.pool, page, h, slot);
     p.pool.positions[i] = (p.seen != nullptr ? p.seen[b] : held) + t;
     p.pool.weights[i] = 0.f;
@@ -261,8 +284,8 @@ __global__ void __launch_bounds__(kKv4QuantThreads)
     kv4_expand_kernel(const __grid_constant__ Kv4ExpandParams p) {
   const Kv4QuantRow row = kv4_quant_row(p.heads, p.tokens);
   if (!row.live) return;
-  const int w = threadIdx.x % kKv4RowThreads, b = row.b, t = row.t, h = row.h;
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
+  const int a = threadIdx.x % kKv4RowThreads, b = row.b, t = row.t, h = row.h;
+  uint4 k[2] = {}, v[2] = {};
   if (t < kv4_count(p.seqs, p.counts, b, p.tokens)) {
     const long long slot = static_cast<long long>(p.seqs.lengths[b]) + t;
     const long long page = kv4_page(p.pool, p.seqs, b, slot);
@@ -271,18 +294,27 @@ __global__ void __launch_bounds__(kKv4QuantThreads)
     } else {
       const uint8_t* block = p.pool.pages + kv4_block_offset(p.pool, page, h, slot);
       const uint8_t* vblock = block + kv4_half_bytes(NG);
-      const int tok = static_cast<int>(slot & 15), at = tok * NG + w / (kKv4RowThreads / NG);
-      const uint32_t kc =
-          reinterpret_cast<const uint32_t*>(block + tok * kKv4RowBytes)[kv4_key_word(w)];
+      const int tok = static_cast<int>(slot & 15), at = tok * NG + a / (kKv4RowThreads / NG);
+      const uint32_t* kr = reinterpret_cast<const uint32_t*>(block + tok * kKv4RowBytes);
       const uint16_t* vr = reinterpret_cast<const uint16_t*>(vblock + tok * kKv4RowBytes);
-      const uint32_t vc = vr[kv4_value_half(2 * w)] |
-                          (static_cast<uint32_t>(vr[kv4_value_half(2 * w + 1)]) << 16);
-      k = kv4_decode8<T>(kc, reinterpret_cast<const uint32_t*>(block + kKv4Block * kKv4RowBytes)[at]);
-      v = kv4_decode8<T>(vc, reinterpret_cast<const uint32_t*>(vblock + kKv4Block * kKv4RowBytes)[at]);
+      const uint32_t kp = reinterpret_cast<const uint32_t*>(block + kKv4Block * kKv4RowBytes)[at];
+      const uint32_t vp = reinterpret_cast<const uint32_t*>(vblock + kKv4Block * kKv4RowBytes)[at];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int w = 2 * a + i;
+        const uint32_t vc = vr[kv4_value_half(2 * w)] |
+                            (static_cast<uint32_t>(vr[kv4_value_half(2 * w + 1)]) << 16);
+        k[i] = kv4_decode8<T>(kr[kv4_key_word(w)], kp);
+        v[i] = kv4_decode8<T>(vc, vp);
+      }
     }
   }
-  *reinterpret_cast<uint4*>(static_cast<T*>(p.k.ptr) + b * p.k.sb + t * p.k.st + h * p.k.sh + 8 * w) = k;
-  *reinterpret_cast<uint4*>(static_cast<T*>(p.v.ptr) + b * p.v.sb + t * p.v.st + h * p.v.sh + 8 * w) = v;
+  uint4* ko = reinterpret_cast<uint4*>(static_cast<T*>(p.k.ptr) + b * p.k.sb + t * p.k.st + h * p.k.sh + 16 * a);
+  uint4* vo = reinterpret_cast<uint4*>(static_cast<T*>(p.v.ptr) + b * p.v.sb + t * p.v.st + h * p.v.sh + 16 * a);
+  ko[0] = k[0];
+  ko[1] = k[1];
+  vo[0] = v[0];
+  vo[1] = v[1];
 }
 
 }  // namespace llmfa
