@@ -108,32 +108,29 @@ int attn_shape(int64_t batch, int64_t heads, int64_t heads_q, int64_t tokens, At
   const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
   const int64_t tiles = (rows + 8 * nt - 1) / (8 * nt);
   *s = AttnShape{batch, heads, heads_q, tokens, nt, static_cast<int>(tiles), batch * heads * tiles};
+  if (s->units * 8 * nt >= (int64_t(1) << 31)) return LLMFA_ERR_UNSUPPORTED;
   return LLMFA_OK;
 }
 
-// CTAs of the attention kernel per SM and their shape.
+// Blocks of the attention kernel on an SM, and their shape.
+template <int WARPS, int STAGES, int CTAS>
+struct AttnShapeOnSm {
+  static constexpr int kWarps = WARPS, kStages = STAGES, kCtas = CTAS, kWorkers = WARPS * CTAS;
+};
 template <int NT>
 struct AttnConfig;
 template <>
-struct AttnConfig<1> {
-  static constexpr int kWarps = 8, kStages = 2, kCtas = 2;
-};
+struct AttnConfig<1> : AttnShapeOnSm<8, 2, 2> {};
 template <>
-struct AttnConfig<2> {
-  static constexpr int kWarps = 12, kStages = 2, kCtas = 1;
-};
+struct AttnConfig<2> : AttnShapeOnSm<12, 2, 1> {};
 template <>
-struct AttnConfig<3> {
-  static constexpr int kWarps = 8, kStages = 3, kCtas = 1;
-};
+struct AttnConfig<3> : AttnShapeOnSm<8, 2, 1> {};
 template <>
-struct AttnConfig<4> {
-  static constexpr int kWarps = 8, kStages = 3, kCtas = 1;
-};
+struct AttnConfig<4> : AttnShapeOnSm<8, 2, 1> {};
 
-int attn_ctas(int nt, int sms) {
-  constexpr int per_sm[] = {AttnConfig<1>::kCtas, AttnConfig<2>::kCtas, AttnConfig<3>::kCtas,
-                            AttnConfig<4>::kCtas};
+int attn_workers(int nt, int sms) {
+  constexpr int per_sm[] = {AttnConfig<1>::kWorkers, AttnConfig<2>::kWorkers, AttnConfig<3>::kWorkers,
+                            AttnConfig<4>::kWorkers};
   return sms * per_sm[nt - 1];
 }
 
@@ -146,7 +143,7 @@ struct AttnLayout {  // byte offsets in the workspace; partial outputs come firs
 constexpr int kMaxSms = 160;
 
 AttnLayout attn_layout(const AttnShape& s) {
-  const uint64_t rows = uint64_t(2) * attn_ctas(s.nt, kMaxSms) * 8 * s.nt;
+  const uint64_t rows = uint64_t(2) * attn_workers(s.nt, kMaxSms) * 8 * s.nt;
   AttnLayout w;
   w.ml = rows * kKv4Dim * sizeof(float);
   w.unit = w.ml + rows * sizeof(float2);
@@ -228,28 +225,27 @@ int select_launch(const Kv4SelectParams& p, long long capacity, int sms, int32_t
 }
 
 template <typename T, int NT, int NG>
-int attn_launch(Kv4AttnParams& p, const AttnShape& shape, int sms, cudaStream_t st) {
+int attn_launch(const Kv4AttnParams& p, const AttnShape& shape, int sms, cudaStream_t st) {
   using C = AttnConfig<NT>;
   constexpr auto kernel = kv4_attention_kernel<T, NT, NG, C::kWarps, C::kStages, C::kCtas>;
   using Smem = Kv4AttnSmem<NT, NG, C::kWarps, C::kStages>;
-  constexpr size_t kMost = sizeof(Smem) + (kKv4MaxBatch + 1) * sizeof(uint32_t);
+  constexpr size_t kMost = sizeof(Smem) + kv4_plan_bytes(kKv4MaxBatch);
   static_assert(kMost <= 227 * 1024, "shared memory");
-  const size_t prefix = static_cast<size_t>(shape.batch + 1) * sizeof(uint32_t);
+  const size_t plan = kv4_plan_bytes(static_cast<int>(shape.batch));
   int rc;
   if ((rc = allow_smem<kernel>(kMost)) != LLMFA_OK) return rc;
-  p.ctas = sms * C::kCtas;
-  kernel<<<static_cast<unsigned>(p.ctas), C::kWarps * 32, sizeof(Smem) + prefix, st>>>(p);
+  kernel<<<static_cast<unsigned>(sms * C::kCtas), C::kWarps * 32, sizeof(Smem) + plan, st>>>(p);
   if ((rc = launched()) != LLMFA_OK) return rc;
-  if ((rc = launch_after(kv4_combine_kernel<T, NT>, static_cast<unsigned>(shape.units),
+  if ((rc = launch_after(kv4_combine_kernel<T, NT>, static_cast<unsigned>(shape.units * 8 * NT),
                          kKv4CombineThreads, 0, st, p)) != LLMFA_OK)
     return rc;
   if (p.row_lse == nullptr) return LLMFA_OK;
   constexpr auto weights = kv4_weights_kernel<T, NT, NG, 8, 3, 2>;
   using WSmem = Kv4WeightsSmem<NT, NG, 8, 3>;
-  constexpr size_t kMostW = sizeof(WSmem) + (kKv4MaxBatch + 1) * sizeof(uint32_t);
-  static_assert(2 * (kMostW + 1024) <= 228 * 1024, "shared memory");
+  constexpr size_t kMostW = sizeof(WSmem) + kv4_plan_bytes(kKv4MaxBatch);
+  static_assert(kMostW <= 227 * 1024, "shared memory");
   if ((rc = allow_smem<weights>(kMostW)) != LLMFA_OK) return rc;
-  return launch_after(weights, static_cast<unsigned>(2 * sms), 8 * 32, sizeof(WSmem) + prefix, st, p);
+  return launch_after(weights, static_cast<unsigned>(2 * sms), 8 * 32, sizeof(WSmem) + plan, st, p);
 }
 
 }  // namespace

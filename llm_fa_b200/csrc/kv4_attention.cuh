@@ -31,10 +31,10 @@
 // The row maximum is lazy: p may reach 2^kKv4Slack before O is rescaled, so a
 // tile needs one vote instead of a reduction over lanes.
 //
-// Each warp has its own ring of tiles in shared memory, filled by bulk copies
-// (a block of 16 tokens is contiguous, keys and values with their pairs): a
-// lane issues them, the warp waits on its own barrier, and warps meet only
-// where a unit ends and their parts are joined.
+// A warp is a worker of its own (kv4_plan.cuh): it has a ring of tiles in
+// shared memory, filled by bulk copies (a block of 16 tokens is contiguous, keys
+// and values with their pairs) that a lane issues and the warp waits for, and
+// writes what it has of a unit. Warps of a block share nothing but the plan.
 #pragma once
 #include <type_traits>
 
@@ -51,13 +51,12 @@ struct Kv4AttnParams {
   float* lse;       // lse[b * lse_sb + h * lse_sh + i], or null
   long long lse_sb, lse_sh;
   const int32_t* counts;
-  float* part_o;   // workspace: [2 * ctas][8 NT][128], fp32
-  float2* part_ml; // [2 * ctas][8 NT]: maximum (log2 units) and sum
-  int2* unit;      // [units]: first CTA of a unit, and how many
+  float* part_o;    // workspace: [2 * workers][8 NT][128], fp32
+  float2* part_ml;  // [2 * workers][8 NT]: maximum (log2 units) and sum
+  int2* unit;       // [units]: first worker of a unit, and how many
   float* row_lse;  // [batch][tokens][heads_q], log2 units; null without tracking
   int heads_q, tokens, causal;
   int group, row_tiles;
-  int ctas;
   float scale_log2;  // softmax_scale * log2(e)
   float decay;       // weights = decay * weights + sums
   unsigned long long timeout_ns;
@@ -164,64 +163,88 @@ __device__ __forceinline__ Kv4Row kv4_row(const Kv4AttnParams& p, int h, int c, 
   return {i, h * p.group + (r - i * p.group), i < c};
 }
 
-// What a segment needs of its query rows, in shared memory.
-template <int NT, int NG>
+// The query rows of a segment, as a lane's B fragments: of n-tile nt, lane (g,
+// c) has of row g the channels 32 j + 8 c .. + 7, the codes of its word j. Step
+// 2j takes nibbles 0, 4 and 1, 5, step 2j + 1 nibbles 2, 6 and 3, 7. Of rows
+// 2c, 2c + 1, whose scores the lane gets, it has the factor and the limit.
+template <int NT>
 struct Kv4Queries {
-  uint2 frag[8][NT][32];    // B fragments of the 8 steps of 16 channels
-  float factor[8 * NT];     // of a score
-  int limit[8 * NT];        // slots that the row sees
-};
+  static constexpr bool kInRegisters = NT <= 2;  // else in the warp's shared memory
+  uint2 frag[8][kInRegisters ? NT : 1];
+  uint2* shared;  // [8][NT][32]
+  float factor[NT][2];
+  int limit[NT][2];  // slots that the row sees
+  int all;           // slots that every live row sees
 
-// One warp prepares the 8 rows of n-tile nt. Step 2j has nibbles 0, 4 (b0) and
-// 1, 5 (b1) of key word j of the lane, step 2j + 1 nibbles 2, 6 and 3, 7: the
-// channels 32 j + 8 c + nibble.
-template <typename T, int NT, int NG>
-__device__ __forceinline__ void kv4_load_queries(const Kv4AttnParams& p, Kv4Queries<NT, NG>& qs,
-                                                 int b, int h, int r0, int n, int c, int nt) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
-  const Kv4Row row = kv4_row(p, h, c, r0 + 8 * nt + g);
-  uint4 raw[4] = {};
-  if (row.live) {
-    const T* q = static_cast<const T*>(p.q.ptr) + b * p.q.sb + row.i * p.q.st + row.hq * p.q.sh;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) raw[j] = *reinterpret_cast<const uint4*>(q + 32 * j + 8 * cc);
+  __device__ __forceinline__ uint2 operator()(int step, int nt) const {
+    if constexpr (kInRegisters) return frag[step][nt];
+    else return shared[(step * NT + nt) * 32 + (threadIdx.x & 31)];
   }
-  float x[4][8], top = 0.f, bad = 0.f;
+
+  template <typename T>
+  __device__ __forceinline__ void load(const Kv4AttnParams& p, int b, int h, int r0, int n, int c) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
+    if constexpr (!kInRegisters) __syncwarp();  // the last segment's are read
+    uint4 raw[NT][4] = {};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t* r = reinterpret_cast<const uint32_t*>(&raw[j]);
+    for (int nt = 0; nt < NT; ++nt) {
+      const Kv4Row row = kv4_row(p, h, c, r0 + 8 * nt + g);
+      if (row.live) {
+        const T* q = static_cast<const T*>(p.q.ptr) + b * p.q.sb + row.i * p.q.st + row.hq * p.q.sh;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 f = Kv4Type<T>::unpack(r[k]);
-      x[j][2 * k] = f.x;
-      x[j][2 * k + 1] = f.y;
-      top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-      bad += f.x * 0.f + f.y * 0.f;  // NaN for NaN and infinities
+        for (int j = 0; j < 4; ++j) raw[nt][j] = *reinterpret_cast<const uint4*>(q + 32 * j + 8 * cc);
+      }
     }
-  }
 #pragma unroll
-  for (int d = 1; d < 4; d <<= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    bad += __shfl_xor_sync(0xffffffffu, bad, d);
-  }
-  // 2^e brings the largest element to [2^13, 2^14)
-  const int e = min(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126);
-  const float up = bad == 0.f ? __int_as_float((e + 127) << 23) : 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      float x[4][8], top = 0.f, bad = 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t y[4];
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t* r = reinterpret_cast<const uint32_t*>(&raw[nt][j]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      y[k] = bad == 0.f ? Kv4Type<__half>::pack(x[j][k] * up, x[j][k + 4] * up) : 0u;
-    qs.frag[2 * j][nt][lane] = make_uint2(y[0], y[1]);
-    qs.frag[2 * j + 1][nt][lane] = make_uint2(y[2], y[3]);
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = Kv4Type<T>::unpack(r[k]);
+          x[j][2 * k] = f.x;
+          x[j][2 * k + 1] = f.y;
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          bad += f.x * 0.f + f.y * 0.f;  // NaN for NaN and infinities
+        }
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        bad += __shfl_xor_sync(0xffffffffu, bad, d);
+      }
+      // 2^e brings the row's largest element to [2^13, 2^14). A row with an infinity or a NaN is
+      // zeros with a NaN factor: it becomes NaN, the others do not.
+      const int e = min(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126);
+      const float up = __int_as_float((e + 127) << 23);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          y[k] = bad == 0.f ? Kv4Type<__half>::pack(x[j][k] * up, x[j][k + 4] * up) : 0u;
+        if constexpr (kInRegisters) {
+          frag[2 * j][nt] = make_uint2(y[0], y[1]);
+          frag[2 * j + 1][nt] = make_uint2(y[2], y[3]);
+        } else {
+          shared[(2 * j * NT + nt) * 32 + lane] = make_uint2(y[0], y[1]);
+          shared[((2 * j + 1) * NT + nt) * 32 + lane] = make_uint2(y[2], y[3]);
+        }
+      }
+      const float f = bad == 0.f ? ldexpf(p.scale_log2, -e) : __int_as_float(0x7fc00000);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        factor[nt][k] = __shfl_sync(0xffffffffu, f, (2 * cc + k) * 4);
+        const Kv4Row row = kv4_row(p, h, c, r0 + 8 * nt + 2 * cc + k);
+        limit[nt][k] = row.live ? kv4_visible(n, c, row.i, p.causal) : 0;
+      }
+    }
+    all = p.causal ? kv4_visible(n, c, r0 / p.group, true) : n;
+    if constexpr (!kInRegisters) __syncwarp();
   }
-  if (cc == 0) {
-    qs.factor[8 * nt + g] =
-        bad == 0.f ? ldexpf(p.scale_log2, -e) : __int_as_float(0x7fc00000);
-    qs.limit[8 * nt + g] = row.live ? kv4_visible(n, c, row.i, p.causal) : 0;
-  }
-}
+};
 
 // ---------------------------------------------------------------- tiles
 // A warp's ring of tiles: STAGES buffers of kKv4TokenBlocks blocks, each of
@@ -265,10 +288,15 @@ struct Kv4Ring {
   }
 };
 
-// Walks the tiles of a CTA's segments that belong to one warp, ahead of the
-// computation, and finds their blocks. Tiles go round the warps.
-// What is needed once a segment stays in shared memory: registers are short.
-template <int WARPS>
+// What a block knows of the sequences, in shared memory.
+struct Kv4Plan {
+  Kv4Split split;
+  const int32_t* held;  // slots of a sequence
+  const int32_t* news;  // its new tokens
+};
+
+// Walks the tiles of a warp's segments ahead of the computation and finds their blocks. What is
+// needed once a segment stays in shared memory: registers are short.
 struct Kv4Loader {
   Kv4Segment* seg;       // this warp's, in shared memory
   const int32_t* table;  // of the segment's sequence
@@ -279,26 +307,19 @@ struct Kv4Loader {
   __device__ __forceinline__ int slot() const {
     return tile * kKv4TileTokens + (threadIdx.x & 31) * kKv4Block;
   }
-  __device__ __forceinline__ void enter(const Kv4AttnParams& p, const Kv4Segment& s, int warp,
-                                        int row_tiles) {
+  __device__ __forceinline__ void enter(const Kv4AttnParams& p, const Kv4Plan& plan,
+                                        const Kv4Segment& s, int row_tiles) {
     if ((threadIdx.x & 31) == 0) *seg = s;
     __syncwarp();
-    tile = s.lo + warp;
+    tile = s.lo;
     hi = s.hi;
-    n = kv4_clamp(p.seqs.lengths[s.b], kv4_capacity(p.pool, p.seqs));
+    n = plan.held[s.b];
     table = p.seqs.table + s.b * p.seqs.table_stride;
     h = s.i / row_tiles;
   }
-  __device__ __forceinline__ void find(const Kv4AttnParams& p, const Kv4Split& split, int warp,
-                                       int row_tiles) {
-    while (more && tile >= hi) {
-      Kv4Segment s = *seg;
-      __syncwarp();
-      more = s.next(split);
-      if (more) enter(p, s, warp, row_tiles);
-    }
+  __device__ __forceinline__ void find(const Kv4AttnParams& p) {
     page = -1;
-    if (more && (threadIdx.x & 31) < kKv4TokenBlocks && slot() < n) {  // n is inside the table
+    if ((threadIdx.x & 31) < kKv4TokenBlocks && slot() < n) {  // n is inside the table
       page = table[slot() >> p.pool.page_shift];
       if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.pool.num_pages)) {
         page = -1;
@@ -306,33 +327,53 @@ struct Kv4Loader {
       }
     }
   }
-  __device__ __forceinline__ void start(const Kv4AttnParams& p, const Kv4Split& split, int cta,
-                                        int warp, int row_tiles) {
-    Kv4Segment s;
-    more = s.first(split, cta);
-    if (more) enter(p, s, warp, row_tiles);
-    find(p, split, warp, row_tiles);
+  __device__ __forceinline__ void start(const Kv4AttnParams& p, const Kv4Plan& plan,
+                                        const Kv4Segment& s, bool any, int row_tiles) {
+    more = any;
+    if (!more) return;
+    enter(p, plan, s, row_tiles);
+    find(p);
   }
   template <typename Ring>
-  __device__ __forceinline__ void issue(const Kv4AttnParams& p, const Kv4Split& split, Ring& ring,
-                                        int warp, int row_tiles) {
+  __device__ __forceinline__ void issue(const Kv4AttnParams& p, const Kv4Plan& plan, Ring& ring,
+                                        int row_tiles) {
     if (!more) return;
     ring.issue(page >= 0 ? p.pool.pages + kv4_block_offset(p.pool, page, h, slot()) : nullptr);
-    tile += WARPS;
-    find(p, split, warp, row_tiles);
+    if (++tile >= hi) {
+      Kv4Segment s = *seg;
+      __syncwarp();
+      more = s.next(plan.split);
+      if (!more) return;
+      enter(p, plan, s, row_tiles);
+    }
+    find(p);
   }
 };
 
-// Costs of the sequences, summed, into shared memory; every CTA does it alike.
+// Bytes of shared memory behind a kernel's own for the plan.
+__host__ __device__ constexpr size_t kv4_plan_bytes(int batch) {
+  return (3 * static_cast<size_t>(batch) + 1) * sizeof(uint32_t);
+}
+// Every block makes the plan alike: the sequences' lengths and costs, summed, into shared memory.
 template <int THREADS>
-__device__ __forceinline__ void kv4_prefix(const Kv4AttnParams& p, uint32_t* prefix) {
+__device__ __forceinline__ void kv4_make_plan(const Kv4AttnParams& p, int hr, uint32_t* space,
+                                              Kv4Plan& plan) {
   __shared__ uint32_t warp_sum[THREADS / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, batch = p.seqs.batch;
+  uint32_t* prefix = space;
+  int32_t* held = reinterpret_cast<int32_t*>(space + batch + 1);
+  int32_t* news = held + batch;
   uint32_t before = 0;
   if (threadIdx.x == 0) prefix[0] = 0;
-  for (int base = 0; base < p.seqs.batch; base += THREADS) {
+  for (int base = 0; base < batch; base += THREADS) {
     const int b = base + threadIdx.x;
-    uint32_t v = b < p.seqs.batch ? kv4_tiles(kv4_length(p.pool, p.seqs, b)) + kKv4UnitCost : 0;
+    uint32_t v = 0;
+    if (b < batch) {
+      const int n = kv4_length(p.pool, p.seqs, b);
+      held[b] = n;
+      news[b] = kv4_count(p.seqs, p.counts, b, p.tokens);
+      v = kv4_tiles(n) + kKv4UnitCost;
+    }
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const uint32_t u = __shfl_up_sync(0xffffffffu, v, d);
@@ -345,15 +386,21 @@ __device__ __forceinline__ void kv4_prefix(const Kv4AttnParams& p, uint32_t* pre
       if (w < warp) add += warp_sum[w];
       before += warp_sum[w];
     }
-    if (b < p.seqs.batch) prefix[b + 1] = v + add;
+    if (b < batch) prefix[b + 1] = v + add;
     __syncthreads();
   }
+  if (threadIdx.x == 0)
+    plan = Kv4Plan{kv4_split(prefix, batch, hr, gridDim.x * (THREADS / 32)), held, news};
+  __syncthreads();
 }
+// Workers next to one another go to different blocks: a small problem uses every SM.
+__device__ __forceinline__ int kv4_worker() { return (threadIdx.x >> 5) * gridDim.x + blockIdx.x; }
 
 // Key codes of 16 tokens times the query rows: x of tokens a (row g of the
 // instruction) and a + 8, in log2 units but for the row factor.
-template <int NT, int NG, typename Frag>
-__device__ __forceinline__ void kv4_scores(uint32_t block, int tok, Frag frag, float (&x)[NT][4]) {
+template <int NT, int NG>
+__device__ __forceinline__ void kv4_scores(uint32_t block, int tok, const Kv4Queries<NT>& q,
+                                           float (&x)[NT][4]) {
   const uint32_t row = block + tok * kKv4RowBytes + (threadIdx.x & 3) * 16;
   const uint4 va = ptx::ld_shared_v4(row), vb = ptx::ld_shared_v4(row + 8 * kKv4RowBytes);
   const uint32_t pairs = block + kKv4Block * kKv4RowBytes + tok * 4 * NG;
@@ -379,7 +426,7 @@ __device__ __forceinline__ void kv4_scores(uint32_t block, int tok, Frag frag, f
         const uint32_t a3 = sixteenth_minus(nibbles_hi(ub), zb.hi);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const uint2 f = frag(2 * j + half, nt);
+          const uint2 f = q(2 * j + half, nt);
           mma_f16(raw[nt], a0, a1, a2, a3, f.x, f.y);
         }
       }
@@ -404,12 +451,10 @@ struct Kv4State {
 };
 
 // One tile of 32 tokens. RAGGED: some row does not see all of it (or a block is
-// missing): `blocks` says which are here, `limit` what each row sees, n what
-// the sequence holds, all counted from the tile's first slot.
-template <typename T, int NT, int NG, bool RAGGED, typename Frag>
-__device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, int tok, Frag frag,
-                                         const float (&factor)[NT][2], uint32_t blocks,
-                                         const int* limit, int slot0, int n) {
+// missing): `blocks` says which are here, n what the sequence holds.
+template <typename T, int NT, int NG, bool RAGGED>
+__device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, int tok,
+                                         const Kv4Queries<NT>& q, uint32_t blocks, int slot0, int n) {
   constexpr bool kTwo = std::is_same<T, __half>::value;  // w in two halves
   constexpr int kBlockBytes = kv4_block_bytes(NG);
   const int lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
@@ -419,7 +464,7 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const uint32_t block = tile + s * kBlockBytes;
-    kv4_scores<NT, NG>(block, tok, frag, x[s]);
+    kv4_scores<NT, NG>(block, tok, q, x[s]);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
       ld_pairs<NG>(block + kv4_half_bytes(NG) + kKv4Block * kKv4RowBytes + (tok + 8 * u) * 4 * NG,
@@ -427,7 +472,7 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[s][nt][k] *= factor[nt][k & 1];
+      for (int k = 0; k < 4; ++k) x[s][nt][k] *= q.factor[nt][k & 1];
     if constexpr (RAGGED) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -441,7 +486,7 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            if (here && slot < limit[8 * nt + 2 * cc + k]) seen |= 1u << (((2 * s + u) * NT + nt) * 2 + k);
+            if (here && slot < q.limit[nt][k]) seen |= 1u << (((2 * s + u) * NT + nt) * 2 + k);
             else x[s][nt][2 * u + k] = -INFINITY;
           }
       }
@@ -580,16 +625,18 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
   }
 }
 
-// 4 channels of a finished row, and with channel 0 its log-sum-exp.
-template <typename T>
+// Channels `at` + 32 k .. + 3 of a finished row, and with channel 0 its log-sum-exp.
+template <typename T, int K>
 __device__ __forceinline__ void kv4_write_row(const Kv4AttnParams& p, int b, int h, int c, int r,
-                                              int at, float4 acc, float m, float l) {
+                                              int at, const float4 (&f)[K], float m, float l) {
   const Kv4Row row = kv4_row(p, h, c, r);
   if (!row.live) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* o = static_cast<T*>(p.o.ptr) + b * p.o.sb + row.i * p.o.st + row.hq * p.o.sh + at;
-  *reinterpret_cast<uint2*>(o) = make_uint2(Kv4Type<T>::pack(acc.x * inv, acc.y * inv),
-                                            Kv4Type<T>::pack(acc.z * inv, acc.w * inv));
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    *reinterpret_cast<uint2*>(o + 32 * k) = make_uint2(Kv4Type<T>::pack(f[k].x * inv, f[k].y * inv),
+                                                       Kv4Type<T>::pack(f[k].z * inv, f[k].w * inv));
   if (at == 0) {
     const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
     if (p.lse != nullptr) p.lse[b * p.lse_sb + row.hq * p.lse_sh + row.i] = lse2 * 0.69314718055994531f;
@@ -597,17 +644,26 @@ __device__ __forceinline__ void kv4_write_row(const Kv4AttnParams& p, int b, int
       p.row_lse[(static_cast<long long>(b) * p.tokens + row.i) * p.heads_q + row.hq] = lse2;
   }
 }
+// Joins a partial result (maximum and sum, output) to another.
+__device__ __forceinline__ void kv4_join(float& m, float& l, float4& acc, float2 ml, float4 f) {
+  const float mn = fmaxf(m, ml.x);
+  // a part without a token has sum and output 0, or NaN: added as it is
+  const float a = m == -INFINITY ? 1.f : ptx::ex2_mufu(m - mn);
+  const float c = ml.x == -INFINITY ? 1.f : ptx::ex2_mufu(ml.x - mn);
+  m = mn;
+  l = fmaf(l, a, ml.y * c);
+  acc.x = fmaf(acc.x, a, f.x * c);
+  acc.y = fmaf(acc.y, a, f.y * c);
+  acc.z = fmaf(acc.z, a, f.z * c);
+  acc.w = fmaf(acc.w, a, f.w * c);
+}
 
 // ---------------------------------------------------------------- the kernel
 template <int NT, int NG, int WARPS, int STAGES>
 struct Kv4AttnSmem {
-  static constexpr int kJoinBlocks = NT == 1 ? 2 : 1;  // blocks of 32 channels joined at a time
-  static constexpr int kJoinRow = 36;                  // floats of a row of 32, free of conflicts
   uint8_t ring[WARPS][STAGES][kKv4TokenBlocks * kv4_block_bytes(NG)];
-  float join[WARPS][kJoinBlocks][8 * NT][kJoinRow];
-  float2 ml[WARPS][8 * NT];
-  Kv4Queries<NT, NG> q;
-  Kv4Split split;
+  uint2 q[Kv4Queries<NT>::kInRegisters ? 1 : WARPS][8 * NT * 32];
+  Kv4Plan plan;
   Kv4Segment seg[WARPS];
   uint64_t bar[WARPS][STAGES];
 };
@@ -619,52 +675,37 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   using Smem = Kv4AttnSmem<NT, NG, WARPS, STAGES>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem_raw + sizeof(Smem));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
 
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) ptx::mbar_init(ptx::smem_u32(&sm.bar[warp][s]), 1);
     ptx::fence_mbar_init();
   }
-  kv4_prefix<kThreads>(p, prefix);
-  if (threadIdx.x == 0) sm.split = kv4_split(prefix, p.seqs.batch, p.pool.heads * p.row_tiles, p.ctas);
-  __syncthreads();
-  const Kv4Split& split = sm.split;
-  const int cta = blockIdx.x;
-  if (cta >= split.parts) return;
+  kv4_make_plan<kThreads>(p, p.pool.heads * p.row_tiles,
+                          reinterpret_cast<uint32_t*>(smem_raw + sizeof(Smem)), sm.plan);
+  const Kv4Plan& plan = sm.plan;
+  const int worker = kv4_worker();
+  Kv4Segment seg;
+  bool more = seg.first(plan.split, worker);
+  if (!more) return;
 
   Kv4Ring<STAGES, kv4_block_bytes(NG)> ring{ptx::smem_u32(sm.ring[warp]),
                                             ptx::smem_u32(sm.bar[warp]), 0, 0, 0};
-  Kv4Loader<WARPS> loader;
+  Kv4Loader loader;
   loader.seg = &sm.seg[warp];
-  loader.start(p, split, cta, warp, p.row_tiles);
-  for (int s = 0; s < STAGES; ++s) loader.issue(p, split, ring, warp, p.row_tiles);
+  loader.start(p, plan, seg, more, p.row_tiles);
+  for (int s = 0; s < STAGES; ++s) loader.issue(p, plan, ring, p.row_tiles);
 
   // rows g and g + 8 of the keys' operand are tokens tok and tok + 8 of a block
   const int tok = (g >> 1) + 4 * (g & 1);
   unsigned long long limit_ns = p.timeout_ns;
-
-  Kv4Segment seg;
-  for (bool more = seg.first(split, cta); more; more = seg.next(split)) {
+  Kv4Queries<NT> q;
+  q.shared = sm.q[Kv4Queries<NT>::kInRegisters ? 0 : warp];
+  for (; more; more = seg.next(plan.split)) {
     const int h = seg.i / p.row_tiles, r0 = (seg.i - h * p.row_tiles) * kRows;
-    const int n = kv4_clamp(p.seqs.lengths[seg.b], kv4_capacity(p.pool, p.seqs));
-    const int c = kv4_count(p.seqs, p.counts, seg.b, p.tokens);
-    if (warp < NT) kv4_load_queries<T, NT, NG>(p, sm.q, seg.b, h, r0, n, c, warp);
-    __syncthreads();
-
-    uint2 qf[NT <= 2 ? 8 : 1][NT];
-    if constexpr (NT <= 2) {
-#pragma unroll
-      for (int s = 0; s < 8; ++s)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) qf[s][nt] = sm.q.frag[s][nt][lane];
-    }
-    auto frag = [&](int s, int nt) {
-      if constexpr (NT <= 2) return qf[s][nt];
-      else return sm.q.frag[s][nt][lane];
-    };
+    const int n = plan.held[seg.b], c = plan.news[seg.b];
+    q.template load<T>(p, seg.b, h, r0, n, c);
     Kv4State<NT, NG> st;
-    float factor[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -675,15 +716,12 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
       for (int k = 0; k < 2; ++k) {
         st.m[nt][k] = -INFINITY;
         st.l[nt][k] = 0.f;
-        factor[nt][k] = sm.q.factor[8 * nt + 2 * cc + k];
       }
     }
 #pragma unroll
     for (int grp = 0; grp < NG; ++grp) st.top[grp] = 127 - 100;
-    // slots below `all` are seen by every live row
-    const int all = p.causal ? kv4_visible(n, c, r0 / p.group, true) : n;
 
-    for (int t = seg.lo + warp; t < seg.hi; t += WARPS) {
+    for (int t = seg.lo; t < seg.hi; ++t) {
       uint32_t blocks = ring.blocks();
       if (!ring.wait(limit_ns)) {
         // The copies never came: report, issue no more, give those in flight a moment each.
@@ -693,126 +731,103 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
         blocks = 0;
       }
       const int slot0 = t * kKv4TileTokens;
-      if (slot0 + kKv4TileTokens > all || blocks != 3u)
-        kv4_tile<T, NT, NG, true>(st, ring.tile(), tok, frag, factor, blocks, sm.q.limit, slot0, n);
+      if (slot0 + kKv4TileTokens > q.all || blocks != 3u)
+        kv4_tile<T, NT, NG, true>(st, ring.tile(), tok, q, blocks, slot0, n);
       else
-        kv4_tile<T, NT, NG, false>(st, ring.tile(), tok, frag, factor, blocks, sm.q.limit, slot0, n);
+        kv4_tile<T, NT, NG, false>(st, ring.tile(), tok, q, blocks, slot0, n);
       ring.release();
-      loader.issue(p, split, ring, warp, p.row_tiles);
+      loader.issue(p, plan, ring, p.row_tiles);
     }
 
-    // ---- join the warps
+    // ---- the warp's piece: the unit's rows, or a slot of the workspace
+    const bool whole = seg.whole();
+    const int slot = 2 * worker + (seg.lo == 0 ? 1 : 0);
+    if (lane == 0 && seg.lo == 0) {
+      const Kv4Pieces pieces = whole ? Kv4Pieces{worker, 1} : kv4_pieces(plan.split, seg.at, seg.tiles);
+      p.unit[seg.b * plan.split.hr + seg.i] = make_int2(pieces.first, pieces.count);
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float l = st.l[nt][k];
+      for (int j = 0; j < 2; ++j) {  // row 2c + j: channels 32 k + 4 g .. + 3
+        float l = st.l[nt][j];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-        if (g == 0) sm.ml[warp][8 * nt + 2 * cc + k] = make_float2(st.m[nt][k], l);
-      }
-    const Kv4Pieces pieces = kv4_pieces(split, seg.at, seg.tiles);
-    const bool whole = pieces.count == 1;
-    const int slot = 2 * cta + (seg.lo == 0 ? 1 : 0);
-    if (threadIdx.x == 0 && seg.lo == 0)
-      p.unit[seg.b * split.hr + seg.i] = make_int2(pieces.first, pieces.count);
-    constexpr int kJoin = Smem::kJoinBlocks;
+        const int r = 8 * nt + 2 * cc + j;
+        float4 f[4];
 #pragma unroll
-    for (int k0 = 0; k0 < 4; k0 += kJoin) {
-#pragma unroll
-      for (int kk = 0; kk < kJoin; ++kk) {
-        const int k = k0 + kk, grp = k * NG / 4;
-        const float back = __int_as_float((st.top[grp] + 1 - kKv4WeightBits) << 23);  // w's factor
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            *reinterpret_cast<float4*>(&sm.join[warp][kk][8 * nt + 2 * cc + j][4 * g]) =
-                make_float4(st.o[2 * k][nt][j] * back, st.o[2 * k][nt][2 + j] * back,
-                            st.o[2 * k + 1][nt][j] * back, st.o[2 * k + 1][nt][2 + j] * back);
-      }
-      __syncthreads();
-      // each thread 4 channels of a row, over the warps
-      for (int e = threadIdx.x; e < kJoin * kRows * 8; e += kThreads) {
-        const int kk = e / (kRows * 8), r = e / 8 % kRows, ch = 4 * (e & 7);
-        float top_m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) top_m = fmaxf(top_m, sm.ml[w][r].x);
-        float sum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-          const float2 ml = sm.ml[w][r];
-          const float a = ml.x == -INFINITY ? 1.f : ptx::ex2_mufu(ml.x - top_m);
-          const float4 f = *reinterpret_cast<const float4*>(&sm.join[w][kk][r][ch]);
-          sum = fmaf(a, ml.y, sum);
-          acc.x = fmaf(a, f.x, acc.x);
-          acc.y = fmaf(a, f.y, acc.y);
-          acc.z = fmaf(a, f.z, acc.z);
-          acc.w = fmaf(a, f.w, acc.w);
+        for (int k = 0; k < 4; ++k) {
+          const float back = __int_as_float((st.top[k * NG / 4] + 1 - kKv4WeightBits) << 23);  // w's factor
+          f[k] = make_float4(st.o[2 * k][nt][j] * back, st.o[2 * k][nt][2 + j] * back,
+                             st.o[2 * k + 1][nt][j] * back, st.o[2 * k + 1][nt][2 + j] * back);
         }
-        const int at = 32 * (k0 + kk) + ch;
-        if (!whole) {
-          *reinterpret_cast<float4*>(p.part_o + (static_cast<long long>(slot) * kRows + r) * kKv4Dim + at) = acc;
-          if (at == 0) p.part_ml[static_cast<long long>(slot) * kRows + r] = make_float2(top_m, sum);
+        if (whole) {
+          kv4_write_row<T, 4>(p, seg.b, h, c, r0 + r, 4 * g, f, st.m[nt][j], l);
         } else {
-          kv4_write_row<T>(p, seg.b, h, c, r0 + r, at, acc, top_m, sum);
+          const long long row = static_cast<long long>(slot) * kRows + r;
+          float4* part = reinterpret_cast<float4*>(p.part_o + row * kKv4Dim + 4 * g);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) part[8 * k] = f[k];
+          if (g == 0) p.part_ml[row] = make_float2(st.m[nt][j], l);
         }
       }
-      __syncthreads();
-    }
   }
 }
 
-// Joins the pieces of the units that were cut: one block a unit, a thread 4
-// channels of a row.
+// Joins the pieces of the units that were cut: one block a unit and row; a
+// warp's lanes have 4 channels each, its pieces are every 8th.
 constexpr int kKv4CombineThreads = 256;
 template <typename T, int NT>
 __global__ void __launch_bounds__(kKv4CombineThreads)
     kv4_combine_kernel(const __grid_constant__ Kv4AttnParams p) {
-  constexpr int kRows = 8 * NT;
+  constexpr int kRows = 8 * NT, kWarps = kKv4CombineThreads / 32;
+  __shared__ float4 acc_of[kWarps][32];
+  __shared__ float2 ml_of[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hr = p.pool.heads * p.row_tiles, u = blockIdx.x / kRows, r = blockIdx.x % kRows;
+  const int b = u / hr, i = u - b * hr, h = i / p.row_tiles, r0 = (i - h * p.row_tiles) * kRows;
+  if (r0 + r >= p.tokens * p.group) return;  // no such row
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int hr = p.pool.heads * p.row_tiles;
-  const int2 unit = p.unit[blockIdx.x];
+  const int2 unit = p.unit[u];
   if (unit.y == 1) return;
-  const int b = blockIdx.x / hr, i = blockIdx.x - b * hr, h = i / p.row_tiles;
-  const int r0 = (i - h * p.row_tiles) * kRows;
-  const int c = kv4_count(p.seqs, p.counts, b, p.tokens);
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = warp; k0 < unit.y; k0 += 4 * kWarps) {
+    float2 ml[4];
+    float4 f[4];
 #pragma unroll
-  for (int e = threadIdx.x; e < kRows * 32; e += kKv4CombineThreads) {
-    const int r = e / 32, at = 4 * (e & 31);
-    float m = -INFINITY;
-    for (int k = 0; k < unit.y; ++k)
-      m = fmaxf(m, p.part_ml[static_cast<long long>(kv4_slot(unit.x, k)) * kRows + r].x);
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = 0; k < unit.y; ++k) {
-      const long long row = static_cast<long long>(kv4_slot(unit.x, k)) * kRows + r;
-      const float2 ml = p.part_ml[row];
-      const float4 f = *reinterpret_cast<const float4*>(p.part_o + row * kKv4Dim + at);
-      const float a = ml.x == -INFINITY ? 1.f : ptx::ex2_mufu(ml.x - m);
-      l = fmaf(a, ml.y, l);
-      acc.x = fmaf(a, f.x, acc.x);
-      acc.y = fmaf(a, f.y, acc.y);
-      acc.z = fmaf(a, f.z, acc.z);
-      acc.w = fmaf(a, f.w, acc.w);
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + j * kWarps;
+      ml[j] = make_float2(-INFINITY, 0.f);
+      f[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < unit.y) {
+        const long long row = static_cast<long long>(kv4_slot(unit.x, k)) * kRows + r;
+        ml[j] = p.part_ml[row];
+        f[j] = *reinterpret_cast<const float4*>(p.part_o + row * kKv4Dim + 4 * lane);
+      }
     }
-    kv4_write_row<T>(p, b, h, c, r0 + r, at, acc, m, l);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kv4_join(m, l, acc, ml[j], f[j]);
   }
+  acc_of[warp][lane] = acc;
+  if (lane == 0) ml_of[warp] = make_float2(m, l);
+  __syncthreads();
+  if (warp != 0) return;
+  for (int w = 1; w < kWarps; ++w) kv4_join(m, l, acc, ml_of[w], acc_of[w][lane]);
+  const float4 f[1] = {acc};
+  kv4_write_row<T, 1>(p, b, h, kv4_count(p.seqs, p.counts, b, p.tokens), r0 + r, 4 * lane, f, m, l);
 }
 
 // The weight that every cached token received: x again, from the keys' half of
 // the cache alone, against the rows' final log-sum-exp. 2^(x - lse) is summed
 // over the rows in a fixed order; row tiles past the first add to what the same
-// thread wrote.
+// lane wrote.
 template <int NT, int NG, int WARPS, int STAGES>
 struct Kv4WeightsSmem {
   uint8_t ring[WARPS][STAGES][kKv4TokenBlocks * kv4_half_bytes(NG)];
-  Kv4Queries<NT, NG> q;
-  float lse[8 * NT];
+  uint2 q[Kv4Queries<NT>::kInRegisters ? 1 : WARPS][8 * NT * 32];
   int page[WARPS][STAGES][kKv4TokenBlocks];
-  Kv4Split split;
+  Kv4Plan plan;
   Kv4Segment seg[WARPS];
   uint64_t bar[WARPS][STAGES];
 };
@@ -824,69 +839,46 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   using Smem = Kv4WeightsSmem<NT, NG, WARPS, STAGES>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem_raw + sizeof(Smem));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) ptx::mbar_init(ptx::smem_u32(&sm.bar[warp][s]), 1);
     ptx::fence_mbar_init();
   }
-  kv4_prefix<kThreads>(p, prefix);
-  if (threadIdx.x == 0) sm.split = kv4_split(prefix, p.seqs.batch, p.pool.heads, gridDim.x);
-  __syncthreads();
-  const Kv4Split& split = sm.split;
-  const int cta = blockIdx.x;
-  if (cta >= split.parts) return;
+  kv4_make_plan<kThreads>(p, p.pool.heads, reinterpret_cast<uint32_t*>(smem_raw + sizeof(Smem)),
+                          sm.plan);
+  const Kv4Plan& plan = sm.plan;
+  Kv4Segment first;
+  if (!first.first(plan.split, kv4_worker())) return;
   Kv4Ring<STAGES, kv4_half_bytes(NG)> ring{ptx::smem_u32(sm.ring[warp]),
                                            ptx::smem_u32(sm.bar[warp]), 0, 0, 0};
-  Kv4Loader<WARPS> loader{};
+  Kv4Loader loader{};
   loader.seg = &sm.seg[warp];
   unsigned long long limit_ns = p.timeout_ns;
   auto issue = [&] {
-    if (loader.more && lane < kKv4TokenBlocks)
-      sm.page[warp][ring.head % STAGES][lane] = loader.page;
-    loader.issue(p, split, ring, warp, 1);
+    if (loader.more && lane < kKv4TokenBlocks) sm.page[warp][ring.head % STAGES][lane] = loader.page;
+    loader.issue(p, plan, ring, 1);
   };
   const int tok = (g >> 1) + 4 * (g & 1);
+  Kv4Queries<NT> q;
+  q.shared = sm.q[Kv4Queries<NT>::kInRegisters ? 0 : warp];
   for (int rt = 0; rt < p.row_tiles; ++rt) {
-    loader.start(p, split, cta, warp, 1);
-    if (limit_ns != p.timeout_ns) loader.more = false;  // after a timeout
+    loader.start(p, plan, first, limit_ns == p.timeout_ns, 1);  // no more after a timeout
     for (int s = 0; s < STAGES; ++s) issue();
     if (rt == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows' log-sum-exp
-    Kv4Segment seg;
-    for (bool more = seg.first(split, cta); more; more = seg.next(split)) {
-      const int h = seg.i, r0 = rt * kRows;
-      const int n = kv4_clamp(p.seqs.lengths[seg.b], kv4_capacity(p.pool, p.seqs));
-      const int c = kv4_count(p.seqs, p.counts, seg.b, p.tokens);
-      __syncthreads();  // the last segment's rows are read
-      if (warp < NT) kv4_load_queries<T, NT, NG>(p, sm.q, seg.b, h, r0, n, c, warp);
-      if (threadIdx.x < kRows) {
-        const Kv4Row row = kv4_row(p, h, c, r0 + threadIdx.x);
-        sm.lse[threadIdx.x] =
-            row.live ? p.row_lse[(static_cast<long long>(seg.b) * p.tokens + row.i) * p.heads_q + row.hq]
-                     : INFINITY;
-      }
-      __syncthreads();
-      uint2 qf[NT <= 2 ? 8 : 1][NT];
-      if constexpr (NT <= 2) {
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) qf[s][nt] = sm.q.frag[s][nt][lane];
-      }
-      auto frag = [&](int s, int nt) {
-        if constexpr (NT <= 2) return qf[s][nt];
-        else return sm.q.frag[s][nt][lane];
-      };
-      float factor[NT][2], lse[NT][2];
+    Kv4Segment seg = first;
+    for (bool more = true; more; more = seg.next(plan.split)) {
+      const int h = seg.i, r0 = rt * kRows, n = plan.held[seg.b], c = plan.news[seg.b];
+      q.template load<T>(p, seg.b, h, r0, n, c);
+      float lse[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int r = 8 * nt + 2 * cc + k;
-          factor[nt][k] = sm.q.factor[r];
-          lse[nt][k] = sm.lse[r];
+          const Kv4Row row = kv4_row(p, h, c, r0 + 8 * nt + 2 * cc + k);
+          lse[nt][k] = row.live ? p.row_lse[(static_cast<long long>(seg.b) * p.tokens + row.i) * p.heads_q + row.hq]
+                                : INFINITY;
         }
-      for (int t = seg.lo + warp; t < seg.hi; t += WARPS) {
+      for (int t = seg.lo; t < seg.hi; ++t) {
         uint32_t blocks = ring.blocks();
         if (!ring.wait(limit_ns)) {
           kv4_report(p.seqs, kStatusTimeout + kSiteKv4Tile);
@@ -899,9 +891,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
         float sum[4];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const uint32_t block = tile + s * kv4_half_bytes(NG);
           float x[NT][4];
-          kv4_scores<NT, NG>(block, tok, frag, x);
+          kv4_scores<NT, NG>(tile + s * kv4_half_bytes(NG), tok, q, x);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int slot = slot0 + 16 * s + tok + 8 * u;
@@ -910,8 +901,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                const float pr = ptx::ex2_mufu(fmaf(x[nt][2 * u + k], factor[nt][k], -lse[nt][k]));
-                w += slot < sm.q.limit[8 * nt + 2 * cc + k] ? pr : 0.f;
+                const float pr = ptx::ex2_mufu(fmaf(x[nt][2 * u + k], q.factor[nt][k], -lse[nt][k]));
+                w += slot < q.limit[nt][k] ? pr : 0.f;
               }
             sum[2 * s + u] = w;
           }

@@ -1,5 +1,5 @@
 // Host run of the 4-bit attention's work split (kv4_plan.cuh): every tile of every unit is in
-// exactly one CTA's segments, pieces are found again with distinct slots, shares are even.
+// exactly one worker's segments, pieces are found again with distinct slots, shares are even.
 #include <cstdio>
 #include <cstdlib>
 #include <map>
@@ -23,11 +23,10 @@ static void run(const std::vector<int>& lens, int hr, int ctas) {
   std::vector<uint32_t> prefix(B + 1, 0);
   for (int b = 0; b < B; ++b) prefix[b + 1] = prefix[b] + kv4_tiles(lens[b]) + kKv4UnitCost;
   const Kv4Split s = kv4_split(prefix.data(), B, hr, ctas);
-  CHECK(s.parts >= 1 && s.parts <= ctas);
+  CHECK(s.share >= kKv4MinShare && s.share * ctas >= s.cost);
+  CHECK(s.share == kKv4MinShare || (s.share - 1) * ctas < s.cost);
   std::map<std::pair<int, int>, std::vector<std::pair<int, Kv4Segment>>> pieces;
-  long long most = 0;
-  for (int c = 0; c < s.parts; ++c) {
-    most = std::max(most, s.bound(c + 1) - s.bound(c));
+  for (int c = 0; c < ctas; ++c) {
     Kv4Segment g{};
     for (bool ok = g.first(s, c); ok; ok = g.next(s)) {
       CHECK(g.b >= 0 && g.b < B && g.i >= 0 && g.i < hr && g.tiles == kv4_tiles(lens[g.b]));
@@ -35,7 +34,6 @@ static void run(const std::vector<int>& lens, int hr, int ctas) {
       pieces[{g.b, g.i}].push_back({c, g});
     }
   }
-  CHECK(most <= (s.cost + s.parts - 1) / s.parts);
   CHECK(static_cast<int>(pieces.size()) == B * hr);
   std::set<int> slots;
   for (auto& [unit, list] : pieces) {
@@ -48,8 +46,9 @@ static void run(const std::vector<int>& lens, int hr, int ctas) {
       at = list[k].second.hi;
       if (p.count > 1) {
         const int slot = kv4_slot(p.first, k);
-        CHECK(slot >= 0 && slot < 2 * s.parts && slots.insert(slot).second);
-        // the slot that the CTA itself derives from its segment
+        CHECK(slot >= 0 && slot < 2 * ctas && slots.insert(slot).second);
+        CHECK(!list[k].second.whole());
+        // the slot that the worker itself derives from its segment
         CHECK(slot == 2 * list[k].first + (list[k].second.lo == 0 ? 1 : 0));
       }
     }
@@ -60,7 +59,7 @@ static void run(const std::vector<int>& lens, int hr, int ctas) {
 int main() {
   unsigned seed = 1;
   auto rnd = [&](int n) { return static_cast<int>((seed = seed * 1664525u + 1013904223u) >> 8) % n; };
-  for (int ctas : {1, 2, 7, 148, 296}) {
+  for (int ctas : {1, 2, 7, 148, 2368}) {
     run({0}, 1, ctas);
     run({1}, 1, ctas);
     run({131071}, 8, ctas);
@@ -79,7 +78,9 @@ int main() {
   std::vector<uint32_t> prefix(B + 1, 0);
   for (int b = 0; b < B; ++b) prefix[b + 1] = prefix[b] + 6000000u + kKv4UnitCost;
   const Kv4Split s = kv4_split(prefix.data(), B, 1024, 296);
-  CHECK(s.cost > (1ll << 40) && s.parts == 296);
+  CHECK(s.cost > (1ll << 40));
+  for (long long x : {0ll, 1ll, s.share - 1, s.share, s.share + 1, 17 * s.share - 1, 17 * s.share, s.cost - 1})
+    CHECK(s.owner(x) == x / s.share);
   long long sum = 0;
   for (int c = 0; c < 296; ++c) {
     Kv4Segment g{};
