@@ -120,7 +120,7 @@ struct AttnShapeOnSm {
 template <int NT>
 struct AttnConfig;
 template <>
-struct AttnConfig<1> : AttnShapeOnSm<8, 2, 2> {};
+struct AttnConfig<1> : AttnShapeOnSm<6, 2, 2> {};
 template <>
 struct AttnConfig<2> : AttnShapeOnSm<12, 2, 1> {};
 template <>
@@ -415,16 +415,14 @@ int llmfa_kv4_evict_move(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seq
   int rc;
   if ((rc = check_cache(cache, seqs, false, &p.pool, &p.seqs)) != LLMFA_OK) return rc;
   if (src == nullptr || keep < 1) return LLMFA_ERR_INVALID_ARGUMENT;
-  if (!aligned(src, 4) || keep >= (int64_t(1) << 31)) return LLMFA_ERR_UNSUPPORTED;
-  const int64_t blocks =
-      (seqs->batch * cache->heads * keep + kKv4MoveThreads - 1) / kKv4MoveThreads;
-  if (blocks >= (int64_t(1) << 31)) return LLMFA_ERR_UNSUPPORTED;
+  if (!aligned(src, 4) || keep > (int64_t(1) << 31) - 1024) return LLMFA_ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>((keep + kKv4MoveThreads - 1) / kKv4MoveThreads),
+                  static_cast<unsigned>(cache->heads), static_cast<unsigned>(seqs->batch));
   if ((rc = device_status_ptr(&p.seqs.status)) != LLMFA_OK) return rc;
   p.src = src;
   p.keep = static_cast<int>(keep);
   return by_type_and_groups(LLMFA_BF16, p.pool.ng, [&](auto, auto ng) {
-    kv4_move_kernel<ng.value><<<static_cast<unsigned>(blocks), kKv4MoveThreads, 0,
-                                static_cast<cudaStream_t>(stream)>>>(p);
+    kv4_move_kernel<ng.value><<<grid, kKv4MoveThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
     return launched();
   });
 }

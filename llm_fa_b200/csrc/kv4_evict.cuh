@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(kKv4SelectThreads)
   }
 }
 
+// ---------------------------------------------------------------- move
 constexpr int kKv4MoveThreads = 256;
 
 struct Kv4MoveParams {
@@ -384,34 +385,79 @@ struct Kv4MoveParams {
   int keep;
 };
 
-// One thread a target slot: copies the token's rows, pairs, position and weight.
 template <int NG>
-__global__ void __launch_bounds__(kKv4MoveThreads) kv4_move_kernel(Kv4MoveParams p) {
-  const long long i = static_cast<long long>(blockIdx.x) * kKv4MoveThreads + threadIdx.x;
-  if (i >= static_cast<long long>(p.seqs.batch) * p.pool.heads * p.keep) return;
-  const int from = p.src[i], to = static_cast<int>(i % p.keep);
-  if (from < 0 || from == to) return;
-  const int bh = static_cast<int>(i / p.keep), h = bh % p.pool.heads, b = bh / p.pool.heads;
-  const long long pf = kv4_page(p.pool, p.seqs, b, from), pt = kv4_page(p.pool, p.seqs, b, to);
-  if (from < p.keep || pf < 0 || pt < 0) {
-    kv4_report(p.seqs, from < p.keep ? kStatusKv4BadSource : kStatusKv4BadPage);
-    return;
+struct Kv4PairWords;
+template <>
+struct Kv4PairWords<1> {
+  using Type = uint32_t;
+};
+template <>
+struct Kv4PairWords<2> {
+  using Type = uint2;
+};
+template <>
+struct Kv4PairWords<4> {
+  using Type = uint4;
+};
+
+// A warp has 32 target slots of one (sequence, head). The lanes whose slot takes
+// another token carry its pairs, position and weight, and list where its rows
+// lie; then 8 lanes carry a token's two rows of 64 bytes, 16 bytes each.
+template <int NG>
+__global__ void __launch_bounds__(kKv4MoveThreads)
+    kv4_move_kernel(const __grid_constant__ Kv4MoveParams p) {
+  __shared__ longlong2 rows[kKv4MoveThreads / 32][32];  // byte offsets: from, to
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int to = (blockIdx.x * kKv4MoveThreads + threadIdx.x);
+  const int h = blockIdx.y, b = blockIdx.z;
+  const long long unit = static_cast<long long>(b) * p.pool.heads + h;
+  const int from = to < p.keep ? p.src[unit * p.keep + to] : -1;
+  bool moves = from >= 0 && from != to;
+  long long pf = -1, pt = -1;
+  if (moves) {
+    pf = kv4_page(p.pool, p.seqs, b, from);
+    pt = kv4_page(p.pool, p.seqs, b, to);
+    if (from < p.keep || pf < 0 || pt < 0) {
+      kv4_report(p.seqs, from < p.keep ? kStatusKv4BadSource : kStatusKv4BadPage);
+      moves = false;
+    }
   }
-  const uint8_t* f = p.pool.pages + kv4_block_offset(p.pool, pf, h, from);
-  uint8_t* t = p.pool.pages + kv4_block_offset(p.pool, pt, h, to);
-  for (int side = 0; side < 2; ++side) {
-    for (int c = 0; c < 4; ++c)
-      reinterpret_cast<uint4*>(t + (to & 15) * kKv4RowBytes)[c] =
-          reinterpret_cast<const uint4*>(f + (from & 15) * kKv4RowBytes)[c];
-    for (int c = 0; c < NG; ++c)
-      reinterpret_cast<uint32_t*>(t + kKv4Block * kKv4RowBytes)[(to & 15) * NG + c] =
-          reinterpret_cast<const uint32_t*>(f + kKv4Block * kKv4RowBytes)[(from & 15) * NG + c];
-    f += kv4_half_bytes(NG);
-    t += kv4_half_bytes(NG);
+  const uint32_t vote = __ballot_sync(0xffffffffu, moves);
+  if (vote == 0) return;
+  if (moves) {
+    using Words = typename Kv4PairWords<NG>::Type;
+    const long long bf = kv4_block_offset(p.pool, pf, h, from), bt = kv4_block_offset(p.pool, pt, h, to);
+    rows[warp][__popc(vote & ((1u << lane) - 1u))] =
+        make_longlong2(bf + (from & 15) * kKv4RowBytes, bt + (to & 15) * kKv4RowBytes);
+    const long long it = kv4_token_index(p.pool, pt, h, to), jf = kv4_token_index(p.pool, pf, h, from);
+    const Words* wf = reinterpret_cast<const Words*>(p.pool.pages + bf + kKv4Block * kKv4RowBytes) + (from & 15);
+    Words* wt = reinterpret_cast<Words*>(p.pool.pages + bt + kKv4Block * kKv4RowBytes) + (to & 15);
+    constexpr int kSide = kv4_half_bytes(NG) / static_cast<int>(sizeof(Words));
+    const Words wk = wf[0], wv = wf[kSide];
+    const int32_t position = p.pool.positions[jf];
+    const float weight = p.pool.weights[jf];
+    wt[0] = wk;
+    wt[kSide] = wv;
+    p.pool.positions[it] = position;
+    p.pool.weights[it] = weight;
   }
-  const long long it = kv4_token_index(p.pool, pt, h, to), jf = kv4_token_index(p.pool, pf, h, from);
-  p.pool.positions[it] = p.pool.positions[jf];
-  p.pool.weights[it] = p.pool.weights[jf];
+  __syncwarp();
+  const int n = __popc(vote), part = lane & 7;
+  const int at = (part & 3) * 16 + (part >> 2) * kv4_half_bytes(NG);
+  for (int i = lane >> 3; i < n; i += 16) {
+    uint4 v[4];
+    longlong2 r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (i + 4 * k < n) {
+        r[k] = rows[warp][i + 4 * k];
+        v[k] = *reinterpret_cast<const uint4*>(p.pool.pages + r[k].x + at);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + 4 * k < n) *reinterpret_cast<uint4*>(p.pool.pages + r[k].y + at) = v[k];
+  }
 }
 
 }  // namespace llmfa
