@@ -264,10 +264,11 @@ int llmfa_kv4_expand(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, v
                      const int64_t k_strides[3], void* v, const int64_t v_strides[3],
                      const int32_t* counts, int64_t tokens, int dtype, void* stream);
 
-/* Workspace of llmfa_kv4_attention, 16-byte aligned. Its contents are not read
- * across calls; calls that share one must not overlap. */
+/* Workspace of llmfa_kv4_attention, 16-byte aligned; capacity is max_pages *
+ * page_size of a call that tracks, else 0. Its contents are not read across
+ * calls; calls that share one must not overlap. */
 int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t heads_q,
-                                       int64_t tokens, uint64_t* bytes);
+                                       int64_t tokens, int64_t capacity, uint64_t* bytes);
 
 /*
  * o = softmax(q k^T * softmax_scale) v for the last counts[b] tokens of each

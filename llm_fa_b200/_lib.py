@@ -95,7 +95,7 @@ SIGNATURES = {
         ctypes.c_void_p, _I64x3, ctypes.c_void_p, _I64x3, ctypes.c_void_p, ctypes.c_int64,
         ctypes.c_int, ctypes.c_void_p]),
     "llmfa_kv4_attention_workspace_size": (ctypes.c_int, [
-        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
         ctypes.POINTER(ctypes.c_uint64)]),
     "llmfa_kv4_attention": (ctypes.c_int, _KV4 + [
         ctypes.c_void_p, _I64x3, ctypes.c_void_p, _I64x3, ctypes.c_void_p,

@@ -135,29 +135,37 @@ int attn_workers(int nt, int sms) {
 }
 
 struct AttnLayout {  // byte offsets in the workspace; partial outputs come first
-  uint64_t ml, unit, row_lse, bytes;
+  uint64_t ml, unit, row_lse, scores, bytes;
 };
+
+// Tracking keeps the scores up to this size, past it the keys are read again. KV4_SCORES
+constexpr uint64_t kMostScores = uint64_t(256) << 20;
 
 // The grid uses at most this many SMs (a B200 has 148), so that the workspace's size follows from
 // a call's arguments alone.
 constexpr int kMaxSms = 160;
 
-AttnLayout attn_layout(const AttnShape& s) {
+// `capacity`: slots of a sequence where the call tracks, else 0.
+AttnLayout attn_layout(const AttnShape& s, int64_t capacity) {
   const uint64_t rows = uint64_t(2) * attn_workers(s.nt, kMaxSms) * 8 * s.nt;
   AttnLayout w;
   w.ml = rows * kKv4Dim * sizeof(float);
   w.unit = w.ml + rows * sizeof(float2);
   w.row_lse = w.unit + static_cast<uint64_t>(s.units) * sizeof(int2);
-  w.bytes = w.row_lse + static_cast<uint64_t>(s.batch * s.heads_q * s.tokens) * sizeof(float);
+  const uint64_t rows_all = static_cast<uint64_t>(s.batch * s.heads_q * s.tokens);
+  w.scores = (w.row_lse + (capacity > 0 ? rows_all * sizeof(float) : 0) + 15) / 16 * 16;
+  const bool keep = capacity > 0 && s.tokens * (s.heads_q / s.heads) <= kKv4SumRows &&
+                    static_cast<uint64_t>(capacity) <= kMostScores / sizeof(float) / rows_all;
+  w.bytes = w.scores + (keep ? rows_all * capacity * sizeof(float) : 0);
   return w;
 }
 
 // A launch that may start while the kernel before it ends, and waits for it itself.
 template <typename K>
-int launch_after(K kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t st,
+int launch_after(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t st,
                  const Kv4AttnParams& p) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -240,6 +248,15 @@ int attn_launch(const Kv4AttnParams& p, const AttnShape& shape, int sms, cudaStr
                          kKv4CombineThreads, 0, st, p)) != LLMFA_OK)
     return rc;
   if (p.row_lse == nullptr) return LLMFA_OK;
+  if (p.scores != nullptr) {
+    // blocks for every SM several times over; each goes on through its head's slots
+    const long long capacity = kv4_capacity(p.pool, p.seqs), heads = shape.batch * shape.heads;
+    const long long most = (capacity + kKv4SumThreads - 1) / kKv4SumThreads;
+    const long long want = (16ll * sms + heads - 1) / heads;
+    const dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(want < most ? want : most));
+    return launch_after(kv4_sum_weights_kernel, grid, kKv4SumThreads,
+                        static_cast<size_t>(p.tokens) * p.group * sizeof(float), st, p);
+  }
   constexpr auto weights = kv4_weights_kernel<T, NT, NG, 8, 3, 2>;
   using WSmem = Kv4WeightsSmem<NT, NG, 8, 3>;
   constexpr size_t kMostW = sizeof(WSmem) + kv4_plan_bytes(kKv4MaxBatch);
@@ -308,11 +325,12 @@ int llmfa_kv4_expand(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, v
 }
 
 int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t heads_q, int64_t tokens,
-                                       uint64_t* bytes) {
-  if (bytes == nullptr) return LLMFA_ERR_INVALID_ARGUMENT;
+                                       int64_t capacity, uint64_t* bytes) {
+  if (bytes == nullptr || capacity < 0) return LLMFA_ERR_INVALID_ARGUMENT;
+  if (capacity >= (int64_t(1) << 31)) return LLMFA_ERR_UNSUPPORTED;
   AttnShape shape;
   const int rc = attn_shape(batch, heads, heads_q, tokens, &shape);
-  if (rc == LLMFA_OK) *bytes = attn_layout(shape).bytes;
+  if (rc == LLMFA_OK) *bytes = attn_layout(shape, capacity).bytes;
   return rc;
 }
 
@@ -344,7 +362,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
   if (seqs->batch * (capacity / kKv4TileTokens + 1 + kKv4UnitCost) >= (int64_t(1) << 32))
     return LLMFA_ERR_UNSUPPORTED;
   if (workspace == nullptr || !aligned(workspace, 16)) return LLMFA_ERR_INVALID_ARGUMENT;
-  const AttnLayout ws = attn_layout(shape);
+  const AttnLayout ws = attn_layout(shape, decay >= 0.f ? capacity : 0);
   if (workspace_bytes < ws.bytes) return LLMFA_ERR_INVALID_ARGUMENT;
   int sms = 0;
   if ((rc = device_status_ptr(&p.seqs.status)) != LLMFA_OK || (rc = device_sms(&sms)) != LLMFA_OK)
@@ -355,6 +373,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
   p.part_ml = reinterpret_cast<float2*>(base + ws.ml);
   p.unit = reinterpret_cast<int2*>(base + ws.unit);
   p.row_lse = decay >= 0.f ? reinterpret_cast<float*>(base + ws.row_lse) : nullptr;
+  p.scores = ws.bytes > ws.scores ? reinterpret_cast<float*>(base + ws.scores) : nullptr;
   p.lse = lse;
   p.counts = counts;
   p.heads_q = static_cast<int>(heads_q);

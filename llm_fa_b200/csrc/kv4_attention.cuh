@@ -54,7 +54,8 @@ struct Kv4AttnParams {
   float* part_o;    // workspace: [2 * workers][8 NT][128], fp32
   float2* part_ml;  // [2 * workers][8 NT]: maximum (log2 units) and sum
   int2* unit;       // [units]: first worker of a unit, and how many
-  float* row_lse;  // [batch][tokens][heads_q], log2 units; null without tracking
+  float* row_lse;   // [batch][tokens][heads_q], log2 units; null without tracking
+  float* scores;    // [batch][heads][capacity][rows], log2 units; null where they are not kept
   int heads_q, tokens, causal;
   int group, row_tiles;
   float scale_log2;  // softmax_scale * log2(e)
@@ -451,10 +452,12 @@ struct Kv4State {
 };
 
 // One tile of 32 tokens. RAGGED: some row does not see all of it (or a block is
-// missing): `blocks` says which are here, n what the sequence holds.
+// missing): `blocks` says which are here, n what the sequence holds. `scores`,
+// if not null, takes the scores of rows r0 .. of the head's `rows`.
 template <typename T, int NT, int NG, bool RAGGED>
 __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, int tok,
-                                         const Kv4Queries<NT>& q, uint32_t blocks, int slot0, int n) {
+                                         const Kv4Queries<NT>& q, uint32_t blocks, int slot0, int n,
+                                         float* scores, int rows, int r0) {
   constexpr bool kTwo = std::is_same<T, __half>::value;  // w in two halves
   constexpr int kBlockBytes = kv4_block_bytes(NG);
   const int lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
@@ -491,6 +494,24 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
           }
       }
     }
+  }
+
+  if (scores != nullptr) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int slot = slot0 + 16 * s + tok + 8 * u;
+        if (slot >= n) continue;
+        float* to = scores + static_cast<long long>(slot) * rows;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int r = r0 + 8 * nt + 2 * cc + k;
+            if (r < rows) to[r] = x[s][nt][2 * u + k];
+          }
+      }
   }
 
   // maxima and value scales: a vote decides whether anything has to be rescaled
@@ -721,6 +742,10 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
 #pragma unroll
     for (int grp = 0; grp < NG; ++grp) st.top[grp] = 127 - 100;
 
+    const int rows = p.tokens * p.group;
+    float* scores = p.scores == nullptr ? nullptr
+                    : p.scores + (static_cast<long long>(seg.b) * p.pool.heads + h) *
+                                     kv4_capacity(p.pool, p.seqs) * rows;
     for (int t = seg.lo; t < seg.hi; ++t) {
       uint32_t blocks = ring.blocks();
       if (!ring.wait(limit_ns)) {
@@ -732,9 +757,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
       }
       const int slot0 = t * kKv4TileTokens;
       if (slot0 + kKv4TileTokens > q.all || blocks != 3u)
-        kv4_tile<T, NT, NG, true>(st, ring.tile(), tok, q, blocks, slot0, n);
+        kv4_tile<T, NT, NG, true>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
       else
-        kv4_tile<T, NT, NG, false>(st, ring.tile(), tok, q, blocks, slot0, n);
+        kv4_tile<T, NT, NG, false>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
       ring.release();
       loader.issue(p, plan, ring, p.row_tiles);
     }
@@ -818,10 +843,45 @@ __global__ void __launch_bounds__(kKv4CombineThreads)
   kv4_write_row<T, 1>(p, b, h, kv4_count(p.seqs, p.counts, b, p.tokens), r0 + r, 4 * lane, f, m, l);
 }
 
-// The weight that every cached token received: x again, from the keys' half of
-// the cache alone, against the rows' final log-sum-exp. 2^(x - lse) is summed
-// over the rows in a fixed order; row tiles past the first add to what the same
-// lane wrote.
+// ---------------------------------------------------------------- tracked weights
+// The weight that a cached token received is the sum over the rows of 2^(x -
+// lse), once the rows' log-sum-exp is final. Where the scores were kept (4
+// bytes a token and row), a thread adds up a token's, in the order of the rows.
+constexpr int kKv4SumThreads = 256;
+constexpr int kKv4SumRows = 8192;  // most rows (their log-sum-exp is in shared memory)
+__global__ void __launch_bounds__(kKv4SumThreads)
+    kv4_sum_weights_kernel(const __grid_constant__ Kv4AttnParams p) {
+  extern __shared__ float lse_of[];  // [rows]
+  const int bh = blockIdx.x, b = bh / p.pool.heads, h = bh - b * p.pool.heads;
+  const int n = kv4_clamp(p.seqs.lengths[b], kv4_capacity(p.pool, p.seqs));
+  const int c = kv4_count(p.seqs, p.counts, b, p.tokens), rows = p.tokens * p.group;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int r = threadIdx.x; r < rows; r += kKv4SumThreads) {
+    const Kv4Row row = kv4_row(p, h, c, r);
+    lse_of[r] = row.live ? p.row_lse[(static_cast<long long>(b) * p.tokens + row.i) * p.heads_q + row.hq]
+                         : INFINITY;
+  }
+  __syncthreads();
+  const long long first = bh * kv4_capacity(p.pool, p.seqs);
+  for (int slot = blockIdx.y * kKv4SumThreads + threadIdx.x; slot < n;
+       slot += gridDim.y * kKv4SumThreads) {
+    const long long page = kv4_page(p.pool, p.seqs, b, slot);
+    if (page < 0) continue;  // reported by the attention
+    const float* x = p.scores + (first + slot) * rows;
+    float sum = 0.f;
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) {
+      const float pr = ptx::ex2_mufu(x[r] - lse_of[r]);
+      // unseen: -inf, and so may the row's lse be; no such row: lse +inf
+      sum += x[r] == -INFINITY || lse_of[r] == INFINITY ? 0.f : pr;
+    }
+    float* w = p.pool.weights + kv4_token_index(p.pool, page, h, slot);
+    *w = p.decay == 0.f ? sum : fmaf(p.decay, *w, sum);
+  }
+}
+
+// Where they would take too much memory, x is worked out again from the keys'
+// half of the cache. Row tiles past the first add to what the same lane wrote.
 template <int NT, int NG, int WARPS, int STAGES>
 struct Kv4WeightsSmem {
   uint8_t ring[WARPS][STAGES][kKv4TokenBlocks * kv4_half_bytes(NG)];

@@ -258,12 +258,13 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
         raise RuntimeError(f"decay must be between 0 and 1, got {decay}")
     n = None if counts is None else _ints(counts, "counts", cache, B)
     if out is None:
-        out = (torch.empty if counts is None else torch.zeros)(shape, dtype=q.dtype,
-                                                               device=cache._device)
+        out = (torch.empty_like if counts is None else torch.zeros_like)(
+            q, memory_format=torch.contiguous_format)
         os = _strides3(out.stride())
     else:
         _, os = _rows(out, "out", cache, B, Hq, like=q)
-    nbytes = _size("llmfa_kv4_attention_workspace_size", B, cache._heads, Hq, T)
+    nbytes = _size("llmfa_kv4_attention_workspace_size", B, cache._heads, Hq, T,
+                   0 if decay < 0 else seqs.max_pages * cache.page_size)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=cache._device)
     lse = ls = None
     if return_lse:

@@ -190,11 +190,18 @@ def test_null_structs_and_workspace_sizes(L):
     assert L.llmfa_kv4_evict_move(c, None, _p(16), 4, None) == BAD
     n = ctypes.c_uint64(0)
     size = L.llmfa_kv4_attention_workspace_size
-    assert size(1, 1, 1, 1, None) == BAD
-    assert size(0, 1, 1, 1, ctypes.byref(n)) == BAD
-    assert size(1, 2, 3, 1, ctypes.byref(n)) == BAD
-    assert size(5000, 1, 1, 1, ctypes.byref(n)) == UNSUP
-    assert size(4096, 8, 64, 1 << 20, ctypes.byref(n)) == UNSUP
+    assert size(1, 1, 1, 1, 0, None) == BAD
+    assert size(0, 1, 1, 1, 0, ctypes.byref(n)) == BAD
+    assert size(1, 2, 3, 1, 0, ctypes.byref(n)) == BAD
+    assert size(1, 1, 1, 1, -1, ctypes.byref(n)) == BAD
+    assert size(5000, 1, 1, 1, 0, ctypes.byref(n)) == UNSUP
+    assert size(4096, 8, 64, 1 << 20, 0, ctypes.byref(n)) == UNSUP
+    # tracking keeps scores of up to 256 MB
+    need = []
+    for capacity in (0, 1 << 20, (1 << 20) + 64):
+        assert size(2, 4, 32, 1, capacity, ctypes.byref(n)) == _lib.LLMFA_OK
+        need.append(n.value)
+    assert need[0] < need[2] < need[1] and need[1] - need[2] == 256 << 20
 
 
 def test_python_surface_refuses_cpu_tensors():

@@ -332,6 +332,29 @@ def test_tracked_weights(lens, T, Hq, H, page, group, decay):
     assert np.array_equal(after[~held], before[~held], equal_nan=True)
 
 
+@pytest.mark.parametrize("T,Hq,group", [(1, 8, 64), (3, 16, 32), (40, 8, 128)])
+def test_tracked_weights_without_room_for_the_scores(T, Hq, group):
+    """A page table so long that the scores are worked out again: the same weights."""
+    lens, H, page = [700, 41], 2, 256
+    cache, table = filled(2, H, lens, page, group, seed=5)
+    wide = torch.full((2, (1 << 23) // page), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    q = randn(2, T, Hq, 128, seed=9)
+    counts = [T, T - 1 if T > 1 else 1]
+    tab = table.cpu().numpy()
+    for tb in (table, wide):
+        cache.weights.fill_(2.0)
+        got = kv4_attention(q, cache, tb, ints(lens), counts=ints(counts), decay=0.5, return_lse=True)
+        assert device_status() == 0
+        w, dx = check_attention(got, q, cache, table, lens, counts)
+        after = cache.weights.double().cpu().numpy()
+        for b, n in enumerate(lens):
+            i = np.arange(n)
+            want = 1.0 + w[b]
+            err = np.abs(after[tab[b, i // page], :, i % page] - want)
+            assert (err <= 2 * dx * w[b] + (T * Hq // H + 3) * 2.0 ** -24 * want).all()
+
+
 def test_attention_strided_views_and_repeated_pages():
     """q and out as slices of wider tensors; two sequences that read the same pages."""
     cache, table = filled(1, 2, [200], 16, 64, seed=3)
