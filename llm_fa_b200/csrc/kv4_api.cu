@@ -91,7 +91,9 @@ int quant_grid(int64_t batch, int64_t tokens, int64_t heads, dim3* grid) {
   return LLMFA_OK;
 }
 
-// Rows of a key head, cut into tiles of 8 nt: the fewest tiles, then the least padding.
+// Rows of a key head, cut into tiles of 8 nt. A pass over the cache takes about 2, 3 and 4 parts of
+// time for 8, 16 and 24 rows (8 x 8192 tokens, 8 heads: 25, 37 and 47 us), which decides; tiles of
+// 32 rows, at 81 us, spill registers and win nowhere.
 struct AttnShape {
   int64_t batch, heads, heads_q, tokens;
   int nt, row_tiles;
@@ -105,8 +107,11 @@ int attn_shape(int64_t batch, int64_t heads, int64_t heads_q, int64_t tokens, At
       batch * heads_q >= (int64_t(1) << 31) / tokens)
     return LLMFA_ERR_UNSUPPORTED;
   const int64_t rows = tokens * (heads_q / heads);
-  const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
-  const int64_t tiles = (rows + 8 * nt - 1) / (8 * nt);
+  int nt = 1;
+  auto tiles_of = [&](int n) { return (rows + 8 * n - 1) / (8 * n); };
+  for (int n = 2; n <= 3; ++n)
+    if (tiles_of(n) * (n + 1) < tiles_of(nt) * (nt + 1)) nt = n;
+  const int64_t tiles = tiles_of(nt);
   *s = AttnShape{batch, heads, heads_q, tokens, nt, static_cast<int>(tiles), batch * heads * tiles};
   if (s->units * 8 * nt >= (int64_t(1) << 31)) return LLMFA_ERR_UNSUPPORTED;
   return LLMFA_OK;
@@ -122,15 +127,12 @@ struct AttnConfig;
 template <>
 struct AttnConfig<1> : AttnShapeOnSm<6, 2, 2> {};
 template <>
-struct AttnConfig<2> : AttnShapeOnSm<12, 2, 1> {};
+struct AttnConfig<2> : AttnShapeOnSm<4, 3, 2> {};
 template <>
-struct AttnConfig<3> : AttnShapeOnSm<8, 2, 1> {};
-template <>
-struct AttnConfig<4> : AttnShapeOnSm<8, 2, 1> {};
+struct AttnConfig<3> : AttnShapeOnSm<4, 2, 2> {};
 
 int attn_workers(int nt, int sms) {
-  constexpr int per_sm[] = {AttnConfig<1>::kWorkers, AttnConfig<2>::kWorkers, AttnConfig<3>::kWorkers,
-                            AttnConfig<4>::kWorkers};
+  constexpr int per_sm[] = {AttnConfig<1>::kWorkers, AttnConfig<2>::kWorkers, AttnConfig<3>::kWorkers};
   return sms * per_sm[nt - 1];
 }
 
@@ -244,8 +246,13 @@ int attn_launch(const Kv4AttnParams& p, const AttnShape& shape, int sms, cudaStr
   if ((rc = allow_smem<kernel>(kMost)) != LLMFA_OK) return rc;
   kernel<<<static_cast<unsigned>(sms * C::kCtas), C::kWarps * 32, sizeof(Smem) + plan, st>>>(p);
   if ((rc = launched()) != LLMFA_OK) return rc;
+  // about as many pieces a unit as there are workers for it, or tiles of the longest sequence
+  const long long tiles = kv4_capacity(p.pool, p.seqs) / kKv4TileTokens + 1;
+  const long long pieces = (sms * C::kWorkers + shape.units - 1) / shape.units;
+  int warps = 1;
+  while (warps < kKv4CombineWarps && 8 * warps < (pieces < tiles ? pieces : tiles)) warps *= 2;
   if ((rc = launch_after(kv4_combine_kernel<T, NT>, static_cast<unsigned>(shape.units * 8 * NT),
-                         kKv4CombineThreads, 0, st, p)) != LLMFA_OK)
+                         warps * 32, 0, st, p)) != LLMFA_OK)
     return rc;
   if (p.row_lse == nullptr) return LLMFA_OK;
   if (p.scores != nullptr) {
@@ -381,6 +388,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
   p.causal = causal != 0;
   p.group = static_cast<int>(heads_q / cache->heads);
   p.row_tiles = shape.row_tiles;
+  p.page_stride = static_cast<uint64_t>(kv4_block_offset(p.pool, 1, 0, 0));
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.decay = decay;
   p.timeout_ns = wait_limit_ns();
@@ -389,8 +397,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
     using T = decltype(t);
     if (shape.nt == 1) return attn_launch<T, 1, ng.value>(p, shape, sms, st);
     if (shape.nt == 2) return attn_launch<T, 2, ng.value>(p, shape, sms, st);
-    if (shape.nt == 3) return attn_launch<T, 3, ng.value>(p, shape, sms, st);
-    return attn_launch<T, 4, ng.value>(p, shape, sms, st);
+    return attn_launch<T, 3, ng.value>(p, shape, sms, st);
   });
 }
 

@@ -58,6 +58,7 @@ struct Kv4AttnParams {
   float* scores;    // [batch][heads][capacity][rows], log2 units; null where they are not kept
   int heads_q, tokens, causal;
   int group, row_tiles;
+  uint64_t page_stride;  // bytes of a page, all heads
   float scale_log2;  // softmax_scale * log2(e)
   float decay;       // weights = decay * weights + sums
   unsigned long long timeout_ns;
@@ -183,12 +184,13 @@ struct Kv4Queries {
   }
 
   template <typename T>
-  __device__ __forceinline__ void load(const Kv4AttnParams& p, int b, int h, int r0, int n, int c) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
-    if constexpr (!kInRegisters) __syncwarp();  // the last segment's are read
-    uint4 raw[NT][4] = {};
+  __device__ __forceinline__ void fetch(const Kv4AttnParams& p, int b, int h, int r0, int c,
+                                        uint4 (&raw)[NT][4]) {
+    const int g = (threadIdx.x & 31) >> 2, cc = threadIdx.x & 3;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) raw[nt][j] = make_uint4(0, 0, 0, 0);
       const Kv4Row row = kv4_row(p, h, c, r0 + 8 * nt + g);
       if (row.live) {
         const T* q = static_cast<const T*>(p.q.ptr) + b * p.q.sb + row.i * p.q.st + row.hq * p.q.sh;
@@ -196,6 +198,13 @@ struct Kv4Queries {
         for (int j = 0; j < 4; ++j) raw[nt][j] = *reinterpret_cast<const uint4*>(q + 32 * j + 8 * cc);
       }
     }
+  }
+
+  template <typename T>
+  __device__ __forceinline__ void set(const Kv4AttnParams& p, int h, int r0, int n, int c,
+                                      const uint4 (&raw)[NT][4]) {
+    const int lane = threadIdx.x & 31, cc = lane & 3;
+    if constexpr (!kInRegisters) __syncwarp();  // the last segment's are read
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float x[4][8], top = 0.f, bad = 0.f;
@@ -301,7 +310,8 @@ struct Kv4Plan {
 struct Kv4Loader {
   Kv4Segment* seg;       // this warp's, in shared memory
   const int32_t* table;  // of the segment's sequence
-  int tile, hi, n, h;
+  const uint8_t* pages;  // the head's part of page 0
+  int tile, hi, n;
   bool more;
   int page;  // of this lane's block of the tile, or -1
 
@@ -316,7 +326,7 @@ struct Kv4Loader {
     hi = s.hi;
     n = plan.held[s.b];
     table = p.seqs.table + s.b * p.seqs.table_stride;
-    h = s.i / row_tiles;
+    pages = p.pool.pages + kv4_block_offset(p.pool, 0, s.i / row_tiles, 0);
   }
   __device__ __forceinline__ void find(const Kv4AttnParams& p) {
     page = -1;
@@ -335,11 +345,14 @@ struct Kv4Loader {
     enter(p, plan, s, row_tiles);
     find(p);
   }
-  template <typename Ring>
+  template <int NG, typename Ring>
   __device__ __forceinline__ void issue(const Kv4AttnParams& p, const Kv4Plan& plan, Ring& ring,
                                         int row_tiles) {
     if (!more) return;
-    ring.issue(page >= 0 ? p.pool.pages + kv4_block_offset(p.pool, page, h, slot()) : nullptr);
+    const int in_page = slot() & ((1 << p.pool.page_shift) - 1);
+    ring.issue(page >= 0 ? pages + static_cast<uint64_t>(page) * p.page_stride +
+                               (in_page >> 4) * kv4_block_bytes(NG)
+                         : nullptr);
     if (++tile >= hi) {
       Kv4Segment s = *seg;
       __syncwarp();
@@ -712,20 +725,30 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
 
   Kv4Ring<STAGES, kv4_block_bytes(NG)> ring{ptx::smem_u32(sm.ring[warp]),
                                             ptx::smem_u32(sm.bar[warp]), 0, 0, 0};
+  Kv4Queries<NT> q;
+  q.shared = sm.q[Kv4Queries<NT>::kInRegisters ? 0 : warp];
+  uint4 raw[NT][4];
+  auto fetch = [&] {
+    const int h = seg.i / p.row_tiles;
+    q.template fetch<T>(p, seg.b, h, (seg.i - h * p.row_tiles) * kRows, plan.news[seg.b], raw);
+  };
+  // Early, while the first tiles are looked up, or a segment's results written, where registers
+  // allow it.
+  constexpr bool kEarly = NT == 1;
+  if (kEarly) fetch();
   Kv4Loader loader;
   loader.seg = &sm.seg[warp];
   loader.start(p, plan, seg, more, p.row_tiles);
-  for (int s = 0; s < STAGES; ++s) loader.issue(p, plan, ring, p.row_tiles);
+  for (int s = 0; s < STAGES; ++s) loader.template issue<NG>(p, plan, ring, p.row_tiles);
 
   // rows g and g + 8 of the keys' operand are tokens tok and tok + 8 of a block
   const int tok = (g >> 1) + 4 * (g & 1);
   unsigned long long limit_ns = p.timeout_ns;
-  Kv4Queries<NT> q;
-  q.shared = sm.q[Kv4Queries<NT>::kInRegisters ? 0 : warp];
-  for (; more; more = seg.next(plan.split)) {
+  while (more) {
     const int h = seg.i / p.row_tiles, r0 = (seg.i - h * p.row_tiles) * kRows;
     const int n = plan.held[seg.b], c = plan.news[seg.b];
-    q.template load<T>(p, seg.b, h, r0, n, c);
+    if (!kEarly) fetch();
+    q.template set<T>(p, h, r0, n, c, raw);
     Kv4State<NT, NG> st;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -761,7 +784,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
       else
         kv4_tile<T, NT, NG, false>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
       ring.release();
-      loader.issue(p, plan, ring, p.row_tiles);
+      loader.template issue<NG>(p, plan, ring, p.row_tiles);
     }
 
     // ---- the warp's piece: the unit's rows, or a slot of the workspace
@@ -796,33 +819,38 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
           if (g == 0) p.part_ml[row] = make_float2(st.m[nt][j], l);
         }
       }
+    more = seg.next(plan.split);
+    if (kEarly && more) fetch();
   }
 }
 
 // Joins the pieces of the units that were cut: one block a unit and row; a
-// warp's lanes have 4 channels each, its pieces are every 8th.
-constexpr int kKv4CombineThreads = 256;
+// warp's lanes have 4 channels each, and the warps take the pieces in turn, 8
+// at once: a long sequence alone is cut into hundreds, whose latency would add
+// up otherwise.
+constexpr int kKv4CombineWarps = 32;  // at most
 template <typename T, int NT>
-__global__ void __launch_bounds__(kKv4CombineThreads)
+__global__ void __launch_bounds__(kKv4CombineWarps * 32)
     kv4_combine_kernel(const __grid_constant__ Kv4AttnParams p) {
-  constexpr int kRows = 8 * NT, kWarps = kKv4CombineThreads / 32;
-  __shared__ float4 acc_of[kWarps][32];
-  __shared__ float2 ml_of[kWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kRows = 8 * NT, kAtOnce = 8;
+  __shared__ float4 acc_of[kKv4CombineWarps][32];
+  __shared__ float2 ml_of[kKv4CombineWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int hr = p.pool.heads * p.row_tiles, u = blockIdx.x / kRows, r = blockIdx.x % kRows;
   const int b = u / hr, i = u - b * hr, h = i / p.row_tiles, r0 = (i - h * p.row_tiles) * kRows;
   if (r0 + r >= p.tokens * p.group) return;  // no such row
+  const int c = kv4_count(p.seqs, p.counts, b, p.tokens);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 unit = p.unit[u];
   if (unit.y == 1) return;
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k0 = warp; k0 < unit.y; k0 += 4 * kWarps) {
-    float2 ml[4];
-    float4 f[4];
+  for (int k0 = warp; k0 < unit.y; k0 += kAtOnce * warps) {
+    float2 ml[kAtOnce];
+    float4 f[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = k0 + j * kWarps;
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int k = k0 + j * warps;
       ml[j] = make_float2(-INFINITY, 0.f);
       f[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (k < unit.y) {
@@ -832,15 +860,15 @@ __global__ void __launch_bounds__(kKv4CombineThreads)
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) kv4_join(m, l, acc, ml[j], f[j]);
+    for (int j = 0; j < kAtOnce; ++j) kv4_join(m, l, acc, ml[j], f[j]);
   }
   acc_of[warp][lane] = acc;
   if (lane == 0) ml_of[warp] = make_float2(m, l);
   __syncthreads();
   if (warp != 0) return;
-  for (int w = 1; w < kWarps; ++w) kv4_join(m, l, acc, ml_of[w], acc_of[w][lane]);
+  for (int w = 1; w < warps; ++w) kv4_join(m, l, acc, ml_of[w], acc_of[w][lane]);
   const float4 f[1] = {acc};
-  kv4_write_row<T, 1>(p, b, h, kv4_count(p.seqs, p.counts, b, p.tokens), r0 + r, 4 * lane, f, m, l);
+  kv4_write_row<T, 1>(p, b, h, c, r0 + r, 4 * lane, f, m, l);
 }
 
 // ---------------------------------------------------------------- tracked weights
@@ -916,7 +944,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   unsigned long long limit_ns = p.timeout_ns;
   auto issue = [&] {
     if (loader.more && lane < kKv4TokenBlocks) sm.page[warp][ring.head % STAGES][lane] = loader.page;
-    loader.issue(p, plan, ring, 1);
+    loader.template issue<NG>(p, plan, ring, 1);
   };
   const int tok = (g >> 1) + 4 * (g & 1);
   Kv4Queries<NT> q;
@@ -928,7 +956,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
     Kv4Segment seg = first;
     for (bool more = true; more; more = seg.next(plan.split)) {
       const int h = seg.i, r0 = rt * kRows, n = plan.held[seg.b], c = plan.news[seg.b];
-      q.template load<T>(p, seg.b, h, r0, n, c);
+      uint4 raw[NT][4];
+      q.template fetch<T>(p, seg.b, h, r0, c, raw);
+      q.template set<T>(p, h, r0, n, c, raw);
       float lse[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
