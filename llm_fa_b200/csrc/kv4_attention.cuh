@@ -263,26 +263,28 @@ template <int STAGES, int BYTES>
 struct Kv4Ring {
   static constexpr int kTileBytes = kKv4TokenBlocks * BYTES;
   uint32_t base, bars;  // shared addresses
-  uint32_t head, tail;  // tiles issued and consumed
-  uint32_t have;        // bit 2 * stage + block: that block was copied
+  uint32_t put = 0, take = 0;  // stages of the next tile to issue and to consume
+  uint32_t pending = 0;        // tiles between them
+  uint32_t parity = 0;         // of `take`'s barrier
+  uint32_t have = 0;           // two bits a pending tile, the next lowest: its blocks that were copied
 
-  // Copies the blocks of a tile; lane k < kKv4TokenBlocks brings block k, if `src` is not null.
-  __device__ __forceinline__ void issue(const uint8_t* src) {
+  // Copies the blocks of a tile; lane k < kKv4TokenBlocks brings block k, where `here`.
+  __device__ __forceinline__ void issue(const uint8_t* src, bool here) {
     const int lane = threadIdx.x & 31;
-    const uint32_t stage = head % STAGES, bar = bars + stage * 8;
-    const uint32_t votes = __ballot_sync(0xffffffffu, lane < kKv4TokenBlocks && src != nullptr);
-    have = (have & ~(3u << (2 * stage))) | (votes << (2 * stage));
+    const uint32_t bar = bars + put * 8, to = base + put * kTileBytes + lane * BYTES;
+    const uint32_t votes = __ballot_sync(0xffffffffu, here);
     if (lane == 0) ptx::mbar_arrive_expect_tx(bar, __popc(votes) * BYTES);
     __syncwarp();
-    if (lane < kKv4TokenBlocks && src != nullptr)
-      ptx::bulk_load(base + stage * kTileBytes + lane * BYTES, src, BYTES, bar);
-    ++head;
+    if (here) ptx::bulk_load(to, src, BYTES, bar);
+    have |= votes << (2 * pending);
+    ++pending;
+    put = put + 1 == STAGES ? 0 : put + 1;
   }
   // Waits for the next tile, at most timeout_ns; false when its copies did not arrive (or were
   // not issued, after an earlier one did not).
   __device__ __forceinline__ bool wait(unsigned long long timeout_ns) {
-    if (tail == head) return false;
-    const uint32_t bar = bars + (tail % STAGES) * 8, parity = (tail / STAGES) & 1;
+    if (pending == 0) return false;
+    const uint32_t bar = bars + take * 8;
     if (ptx::mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = ptx::globaltimer_ns();
     for (uint32_t it = 1;; ++it) {
@@ -290,11 +292,17 @@ struct Kv4Ring {
       if ((it & 63u) == 0 && ptx::globaltimer_ns() - t0 > timeout_ns) return false;
     }
   }
-  __device__ __forceinline__ uint32_t tile() const { return base + (tail % STAGES) * kTileBytes; }
-  __device__ __forceinline__ uint32_t blocks() const { return (have >> (2 * (tail % STAGES))) & 3u; }
+  __device__ __forceinline__ uint32_t tile() const { return base + take * kTileBytes; }
+  __device__ __forceinline__ uint32_t blocks() const { return have & 3u; }
   __device__ __forceinline__ void release() {
     __syncwarp();  // every lane has read the tile
-    tail += tail != head;
+    if (pending == 0) return;
+    --pending;
+    have >>= 2;
+    if (++take == STAGES) {
+      take = 0;
+      parity ^= 1u;
+    }
   }
 };
 
@@ -311,27 +319,25 @@ struct Kv4Loader {
   Kv4Segment* seg;       // this warp's, in shared memory
   const int32_t* table;  // of the segment's sequence
   const uint8_t* pages;  // the head's part of page 0
-  int tile, hi, n;
+  int slot, left, n;     // first slot of this lane's block of the tile; tiles left of the segment
   bool more;
-  int page;  // of this lane's block of the tile, or -1
+  int page;  // of the block, or -1: lanes below kKv4TokenBlocks have one
 
-  __device__ __forceinline__ int slot() const {
-    return tile * kKv4TileTokens + (threadIdx.x & 31) * kKv4Block;
-  }
   __device__ __forceinline__ void enter(const Kv4AttnParams& p, const Kv4Plan& plan,
                                         const Kv4Segment& s, int row_tiles) {
     if ((threadIdx.x & 31) == 0) *seg = s;
     __syncwarp();
-    tile = s.lo;
-    hi = s.hi;
-    n = plan.held[s.b];
+    const int lane = threadIdx.x & 31;
+    slot = s.lo * kKv4TileTokens + lane * kKv4Block;
+    left = s.hi - s.lo;
+    n = lane < kKv4TokenBlocks ? plan.held[s.b] : 0;
     table = p.seqs.table + s.b * p.seqs.table_stride;
     pages = p.pool.pages + kv4_block_offset(p.pool, 0, s.i / row_tiles, 0);
   }
   __device__ __forceinline__ void find(const Kv4AttnParams& p) {
     page = -1;
-    if ((threadIdx.x & 31) < kKv4TokenBlocks && slot() < n) {  // n is inside the table
-      page = table[slot() >> p.pool.page_shift];
+    if (slot < n) {  // n is inside the table
+      page = table[slot >> p.pool.page_shift];
       if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.pool.num_pages)) {
         page = -1;
         kv4_report(p.seqs, kStatusKv4BadPage);
@@ -349,11 +355,11 @@ struct Kv4Loader {
   __device__ __forceinline__ void issue(const Kv4AttnParams& p, const Kv4Plan& plan, Ring& ring,
                                         int row_tiles) {
     if (!more) return;
-    const int in_page = slot() & ((1 << p.pool.page_shift) - 1);
-    ring.issue(page >= 0 ? pages + static_cast<uint64_t>(page) * p.page_stride +
-                               (in_page >> 4) * kv4_block_bytes(NG)
-                         : nullptr);
-    if (++tile >= hi) {
+    const int block = (slot & ((1 << p.pool.page_shift) - 1)) >> 4;
+    ring.issue(pages + static_cast<uint64_t>(page) * p.page_stride + block * kv4_block_bytes(NG),
+               page >= 0);
+    slot += kKv4TileTokens;
+    if (--left == 0) {
       Kv4Segment s = *seg;
       __syncwarp();
       more = s.next(plan.split);
@@ -724,7 +730,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   if (!more) return;
 
   Kv4Ring<STAGES, kv4_block_bytes(NG)> ring{ptx::smem_u32(sm.ring[warp]),
-                                            ptx::smem_u32(sm.bar[warp]), 0, 0, 0};
+                                            ptx::smem_u32(sm.bar[warp])};
   Kv4Queries<NT> q;
   q.shared = sm.q[Kv4Queries<NT>::kInRegisters ? 0 : warp];
   uint4 raw[NT][4];
@@ -938,12 +944,12 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   Kv4Segment first;
   if (!first.first(plan.split, kv4_worker())) return;
   Kv4Ring<STAGES, kv4_half_bytes(NG)> ring{ptx::smem_u32(sm.ring[warp]),
-                                           ptx::smem_u32(sm.bar[warp]), 0, 0, 0};
+                                           ptx::smem_u32(sm.bar[warp])};
   Kv4Loader loader{};
   loader.seg = &sm.seg[warp];
   unsigned long long limit_ns = p.timeout_ns;
   auto issue = [&] {
-    if (loader.more && lane < kKv4TokenBlocks) sm.page[warp][ring.head % STAGES][lane] = loader.page;
+    if (loader.more && lane < kKv4TokenBlocks) sm.page[warp][ring.put][lane] = loader.page;
     loader.template issue<NG>(p, plan, ring, 1);
   };
   const int tok = (g >> 1) + 4 * (g & 1);
@@ -1006,7 +1012,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
         const float mine = cc == 0 ? sum[0] : cc == 1 ? sum[1] : cc == 2 ? sum[2] : sum[3];
         const int s = cc >> 1, slot = slot0 + 16 * s + tok + 8 * (cc & 1);
         if (((blocks >> s) & 1u) != 0 && slot < n) {
-          const int page = sm.page[warp][ring.tail % STAGES][s];
+          const int page = sm.page[warp][ring.take][s];
           float* w = p.pool.weights + kv4_token_index(p.pool, page, h, slot);
           *w = rt > 0 ? *w + mine : p.decay == 0.f ? mine : fmaf(p.decay, *w, mine);
         }
