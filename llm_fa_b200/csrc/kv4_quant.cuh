@@ -68,6 +68,11 @@ struct Kv4Type<__nv_bfloat16> {
     asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
 };
 template <>
 struct Kv4Type<__half> {
@@ -81,6 +86,11 @@ struct Kv4Type<__half> {
   static __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
 };
@@ -137,20 +147,17 @@ __device__ __forceinline__ uint32_t kv4_codes(const uint4& raw, const Kv4Pair& p
   return w;
 }
 // lo = min(0, x) and hi = max(0, x) of a group, over the 8 / NG threads that hold it; a NaN in it
-// makes one of them NaN. Both are minima: of x, and of -x with its sign bits flipped.
+// makes both NaN. From thread to thread they go as one word, (lo, -hi): both are minima then.
 template <typename T, int NG>
 __device__ __forceinline__ float2 kv4_range(const uint4 (&raw)[2]) {
-  constexpr uint32_t kSigns = 0x80008000u;
   using V = Kv4Type<T>;
-  uint32_t both = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t lo2 = V::min2(V::min2(raw[i].x, raw[i].y), V::min2(raw[i].z, raw[i].w));
-    const uint32_t hi2 = V::min2(V::min2(raw[i].x ^ kSigns, raw[i].y ^ kSigns),
-                                 V::min2(raw[i].z ^ kSigns, raw[i].w ^ kSigns));
-    // (lo, -hi) of the thread, then of the group
-    both = V::min2(both, V::min2(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632)));
-  }
+  const uint32_t lo2 = V::min2(V::min2(V::min2(raw[0].x, raw[0].y), V::min2(raw[0].z, raw[0].w)),
+                               V::min2(V::min2(raw[1].x, raw[1].y), V::min2(raw[1].z, raw[1].w)));
+  const uint32_t hi2 = V::max2(V::max2(V::max2(raw[0].x, raw[0].y), V::max2(raw[0].z, raw[0].w)),
+                               V::max2(V::max2(raw[1].x, raw[1].y), V::max2(raw[1].z, raw[1].w)));
+  const uint32_t minus = hi2 ^ 0x80008000u;
+  uint32_t both = V::min2(__byte_perm(lo2, minus, 0x5410), __byte_perm(lo2, minus, 0x7632));
+  both = V::min2(both, 0u);
 #pragma unroll
   for (int d = 1; d < kKv4RowThreads / NG; d <<= 1)
     both = V::min2(both, __shfl_xor_sync(0xffffffffu, both, d));
@@ -294,27 +301,28 @@ __global__ void __launch_bounds__(kKv4QuantThreads)
     } else {
       const uint8_t* block = p.pool.pages + kv4_block_offset(p.pool, page, h, slot);
       const uint8_t* vblock = block + kv4_half_bytes(NG);
-      const int tok = static_cast<int>(slot & 15), at = tok * NG + a / (kKv4RowThreads / NG);
+      const int tok = static_cast<int>(slot & 15);
       const uint32_t* kr = reinterpret_cast<const uint32_t*>(block + tok * kKv4RowBytes);
       const uint16_t* vr = reinterpret_cast<const uint16_t*>(vblock + tok * kKv4RowBytes);
-      const uint32_t kp = reinterpret_cast<const uint32_t*>(block + kKv4Block * kKv4RowBytes)[at];
-      const uint32_t vp = reinterpret_cast<const uint32_t*>(vblock + kKv4Block * kKv4RowBytes)[at];
+      const uint32_t* kp = reinterpret_cast<const uint32_t*>(block + kKv4Block * kKv4RowBytes) + tok * NG;
+      const uint32_t* vp = reinterpret_cast<const uint32_t*>(vblock + kKv4Block * kKv4RowBytes) + tok * NG;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int w = 2 * a + i;
+        const int w = a + 8 * i;
         const uint32_t vc = vr[kv4_value_half(2 * w)] |
                             (static_cast<uint32_t>(vr[kv4_value_half(2 * w + 1)]) << 16);
-        k[i] = kv4_decode8<T>(kr[kv4_key_word(w)], kp);
-        v[i] = kv4_decode8<T>(vc, vp);
+        k[i] = kv4_decode8<T>(kr[kv4_key_word(w)], kp[w * NG / 16]);
+        v[i] = kv4_decode8<T>(vc, vp[w * NG / 16]);
       }
     }
   }
-  uint4* ko = reinterpret_cast<uint4*>(static_cast<T*>(p.k.ptr) + b * p.k.sb + t * p.k.st + h * p.k.sh + 16 * a);
-  uint4* vo = reinterpret_cast<uint4*>(static_cast<T*>(p.v.ptr) + b * p.v.sb + t * p.v.st + h * p.v.sh + 16 * a);
+  // words a and a + 8: the 8 threads write 128 contiguous bytes at a time
+  uint4* ko = reinterpret_cast<uint4*>(static_cast<T*>(p.k.ptr) + b * p.k.sb + t * p.k.st + h * p.k.sh + 8 * a);
+  uint4* vo = reinterpret_cast<uint4*>(static_cast<T*>(p.v.ptr) + b * p.v.sb + t * p.v.st + h * p.v.sh + 8 * a);
   ko[0] = k[0];
-  ko[1] = k[1];
+  ko[8] = k[1];
   vo[0] = v[0];
-  vo[1] = v[1];
+  vo[8] = v[1];
 }
 
 }  // namespace llmfa
