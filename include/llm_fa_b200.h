@@ -189,15 +189,15 @@ int llmfa_selftest_wait_timeout(uint32_t timeout_us, void* stream);
  * A paged cache that holds keys and values in 4 bits, attention over it, and
  * eviction from it by the attention weight that its tokens received. Head dim
  * 128; no counterpart in the reference. All calls are stream-ordered, allocate
- * nothing and can be captured in a CUDA graph (after one eager call of any
- * entry point on the device).
+ * nothing and can be captured in a CUDA graph (after one eager call of the same
+ * entry point, type, group and head counts on the device).
  *
  * Device data is not readable before the launch, so what it may hold wrong is
  * found by the kernels and reported in the device status word
  * (llmfa_device_status): a page id outside the pool or a token without a page
  * (the token is not written, counts as absent, or reads as zeros), a length or
- * count outside its range (clamped), a move from outside the sequence (not
- * made).
+ * count outside its range (clamped; nothing is appended behind a negative
+ * length), a move from outside the sequence (not made).
  */
 #define LLMFA_DEVICE_STATUS_KV4_BAD_PAGE 0x2001
 #define LLMFA_DEVICE_STATUS_KV4_BAD_LENGTH 0x2002
@@ -225,7 +225,7 @@ typedef struct llmfa_kv4_cache {
   int32_t group;
 } llmfa_kv4_cache;
 
-/* The sequences of a call (at most 4096): slot i of sequence b is in page
+/* The sequences of a call (at most 4096, of fewer than 2^30 slots): slot i of sequence b is in page
  * page_table[b * table_stride + i / page_size]. lengths[b] slots hold tokens.
  * No two sequences may share a page that a call writes. */
 typedef struct llmfa_kv4_seqs {
@@ -274,7 +274,7 @@ int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t hea
  * o = softmax(q k^T * softmax_scale) v for the last counts[b] tokens of each
  * sequence (counts = NULL: all `tokens`); q, o are [batch, tokens, heads_q,
  * 128], heads_q a multiple of the cache's heads, query head i reading key head
- * i / (heads_q / heads). seqs->lengths counts the new tokens, whose keys are
+ * i / (heads_q / heads); o may not alias q. seqs->lengths counts the new tokens, whose keys are
  * appended already. With causal != 0, new token i sees slots 0 .. lengths[b] -
  * counts[b] + i, else all. A row that sees no slot gets zeros (and lse -inf);
  * rows past a count are left as they were. lse as for llmfa_forward_lse, or

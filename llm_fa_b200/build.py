@@ -27,15 +27,20 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB = PKG / "libllm_fa_b200.so"
-SOURCES = [CSRC / "llm_fa_api.cu", CSRC / "kv4_api.cu"]
-DEPS = (SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
+# The 4-bit cache has no variants: it is compiled once, and every library links the object.
+KV4_SOURCE = CSRC / "kv4_api.cu"
+KV4_OBJECT = PKG / "kv4_api.o"
+KV4_DEPS = ([KV4_SOURCE, CSRC / "ptx.cuh"] + sorted(CSRC.glob("kv4_*.cuh"))
+            + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h")))
+SOURCES = [CSRC / "llm_fa_api.cu"]
+DEPS = (SOURCES + [KV4_SOURCE] + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
         + sorted(INCLUDE.glob("*.h")))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
-    "-Xptxas", "-v", "-split-compile=0",
+    "-Xcompiler", "-fPIC",
+    "-Xptxas", "-v",
 ]
 
 
@@ -75,14 +80,21 @@ def is_stale(lib: Path = LIB, deps: list[Path] = DEPS) -> bool:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile the product library if it is missing or older than its sources."""
-    return _compile(LIB, [], force, verbose)
+    _build_kv4(force, verbose)
+    return _compile(LIB, [], force, verbose, objects=[KV4_OBJECT])
 
 
 def build_variant(name: str, force: bool = False, verbose: bool = False) -> Path:
     """Compile one variant library (see VARIANTS) if missing or stale."""
     if name not in VARIANTS:
         raise ValueError(f"unknown variant {name!r}; one of {sorted(VARIANTS)}")
-    return _compile(variant_path(name), VARIANTS[name], force, verbose)
+    _build_kv4(force and not KV4_OBJECT.exists(), verbose)
+    return _compile(variant_path(name), VARIANTS[name], force, verbose, objects=[KV4_OBJECT])
+
+
+def _build_kv4(force: bool, verbose: bool) -> Path:
+    return _compile(KV4_OBJECT, ["-split-compile=0"], force, verbose, [KV4_SOURCE], KV4_DEPS,
+                    kind="-c")
 
 
 def build_mmarate(force: bool = False, verbose: bool = False) -> Path:
@@ -94,19 +106,24 @@ def build_all(force: bool = False, verbose: bool = False) -> list[Path]:
     """The product library, every variant and the microbenchmark, compiled concurrently
     (one nvcc each)."""
     import concurrent.futures
-    jobs = [(LIB, [], SOURCES, DEPS)] + [(variant_path(n), d, SOURCES, DEPS)
-                                         for n, d in VARIANTS.items()]
-    jobs.append((MMARATE_LIB, [], MMARATE_SOURCES, MMARATE_DEPS))
+    _build_kv4(force, verbose)
+    kv4 = [KV4_OBJECT]
+    jobs = [(LIB, [], SOURCES, DEPS, kv4)] + [(variant_path(n), d, SOURCES, DEPS, kv4)
+                                              for n, d in VARIANTS.items()]
+    jobs.append((MMARATE_LIB, [], MMARATE_SOURCES, MMARATE_DEPS, []))
     with concurrent.futures.ThreadPoolExecutor(max_workers=len(jobs)) as pool:
-        return list(pool.map(lambda j: _compile(j[0], j[1], force, verbose, j[2], j[3]), jobs))
+        return list(pool.map(lambda j: _compile(j[0], j[1], force, verbose, j[2], j[3],
+                                                objects=j[4]), jobs))
 
 
 def _compile(lib: Path, defines: list[str], force: bool, verbose: bool,
-             sources: list[Path] = SOURCES, deps: list[Path] = DEPS) -> Path:
+             sources: list[Path] = SOURCES, deps: list[Path] = DEPS, *,
+             objects: list[Path] = [], kind: str = "-shared") -> Path:
     if not force and not is_stale(lib, deps):
         return lib
     tmp = lib.with_name(lib.name + f".{os.getpid()}.tmp")
-    cmd = [nvcc_path(), *NVCC_FLAGS, *defines, "-o", str(tmp), *map(str, sources)]
+    cmd = [nvcc_path(), *NVCC_FLAGS, kind, *defines, "-o", str(tmp), *map(str, sources),
+           *map(str, objects)]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or proc.returncode != 0:
         sys.stderr.write(proc.stdout + proc.stderr)

@@ -38,7 +38,7 @@ int check_cache(const llmfa_kv4_cache* c, const llmfa_kv4_seqs* s, bool lengths,
       !aligned(s->page_table, 4) || !aligned(s->lengths, 4))
     return LLMFA_ERR_UNSUPPORTED;
   if (c->num_pages >= (int64_t(1) << 31) || c->heads > 1024 || s->batch > kKv4MaxBatch ||
-      s->max_pages >= (int64_t(1) << (31 - shift)) || s->table_stride >= (int64_t(1) << 38))
+      s->max_pages >= (int64_t(1) << (30 - shift)) || s->table_stride >= (int64_t(1) << 38))
     return LLMFA_ERR_UNSUPPORTED;
   *pool = Kv4Pool{static_cast<uint8_t*>(c->pages), c->positions, c->weights, c->num_pages,
                   c->heads, shift, kKv4Dim / c->group};
@@ -140,7 +140,8 @@ struct AttnLayout {  // byte offsets in the workspace; partial outputs come firs
   uint64_t ml, unit, row_lse, scores, bytes;
 };
 
-// Tracking keeps the scores up to this size, past it the keys are read again. KV4_SCORES
+// Tracking keeps the scores up to this size; past it the keys are read again. Kept, 16 sequences of
+// 4097 tokens with 32 heads of one row (8 MB) are tracked in 15 us, read again in 50.
 constexpr uint64_t kMostScores = uint64_t(256) << 20;
 
 // The grid uses at most this many SMs (a B200 has 148), so that the workspace's size follows from
@@ -334,7 +335,7 @@ int llmfa_kv4_expand(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, v
 int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t heads_q, int64_t tokens,
                                        int64_t capacity, uint64_t* bytes) {
   if (bytes == nullptr || capacity < 0) return LLMFA_ERR_INVALID_ARGUMENT;
-  if (capacity >= (int64_t(1) << 31)) return LLMFA_ERR_UNSUPPORTED;
+  if (capacity >= (int64_t(1) << 30)) return LLMFA_ERR_UNSUPPORTED;
   AttnShape shape;
   const int rc = attn_shape(batch, heads, heads_q, tokens, &shape);
   if (rc == LLMFA_OK) *bytes = attn_layout(shape, capacity).bytes;

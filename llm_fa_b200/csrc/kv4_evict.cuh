@@ -186,8 +186,8 @@ __device__ __forceinline__ uint32_t kv4_votes(const uint32_t (&vote)[4]) {
 template <bool SMEM>
 __global__ void __launch_bounds__(kKv4SelectThreads)
     kv4_select_kernel(const __grid_constant__ Kv4SelectParams p, int32_t* movers, int ctas) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  Kv4SelectSmem& sm = *reinterpret_cast<Kv4SelectSmem*>(smem_raw);
+  extern __shared__ __align__(16) uint8_t select_smem[];
+  Kv4SelectSmem& sm = *reinterpret_cast<Kv4SelectSmem*>(select_smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t rank = ptx::cluster_ctarank();
   const int bh = blockIdx.x / ctas, h = bh % p.pool.heads, b = bh / p.pool.heads;
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kKv4SelectThreads)
   const int run = kv4_select_run(n, ctas);
   const int rows = run / kKv4SelectRow;  // of a warp; its rows are consecutive
   const int slot0 = rank * run + (warp * rows) * 128 + 4 * lane;
-  uint32_t* masks = reinterpret_cast<uint32_t*>(smem_raw + sizeof(Kv4SelectSmem)) + warp * rows * 4;
-  uint4* keys = reinterpret_cast<uint4*>(smem_raw + sizeof(Kv4SelectSmem) + run / 8) +
+  uint32_t* masks = reinterpret_cast<uint32_t*>(select_smem + sizeof(Kv4SelectSmem)) + warp * rows * 4;
+  uint4* keys = reinterpret_cast<uint4*>(select_smem + sizeof(Kv4SelectSmem) + run / 8) +
                 warp * rows * 32 + lane;
   auto keys_at = [&](int r) {  // of row r's four slots of this lane
     return SMEM ? keys[r * 32] : kv4_slot_keys(p, table, h, slot0 + r * 128, n, first_recent);

@@ -197,6 +197,10 @@ __global__ void __launch_bounds__(kKv4QuantThreads)
   const int held = p.seqs.lengths[b];
   const long long slot = static_cast<long long>(held) + t;
   bool live = row.live && t < kv4_count(p.seqs, p.counts, b, p.tokens);
+  if (held < 0) {  // no slot to write behind
+    kv4_report(p.seqs, kStatusKv4BadLength);
+    live = false;
+  }
   long long page = -1;
   uint4 raw[2][2] = {};
   if (live) {

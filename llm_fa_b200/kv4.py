@@ -263,6 +263,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
         os = _strides3(out.stride())
     else:
         _, os = _rows(out, "out", cache, B, Hq, like=q)
+        if out.data_ptr() == q.data_ptr():
+            raise RuntimeError("out must not be q itself")
     nbytes = _size("llmfa_kv4_attention_workspace_size", B, cache._heads, Hq, T,
                    0 if decay < 0 else seqs.max_pages * cache.page_size)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=cache._device)
@@ -272,7 +274,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
         ls = _lib.strides2((Hq * T, T))
     _call(cache, "llmfa_kv4_attention", seqs, q.data_ptr(), qs, out.data_ptr(), os,
           lse.data_ptr() if return_lse else None, ls, n, Hq, T, bool(causal),
-          _SCALE if softmax_scale is None else softmax_scale, decay, _DTYPES[q.dtype],
+          _SCALE if softmax_scale is None else float(softmax_scale), decay, _DTYPES[q.dtype],
           ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 

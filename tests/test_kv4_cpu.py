@@ -130,7 +130,7 @@ SHARED = [
     (dict(table_stride=3), BAD), (dict(pages=24), UNSUP), (dict(positions=18), UNSUP),
     (dict(weights=18), UNSUP), (dict(page_table=18), UNSUP), (dict(heads=2000), UNSUP),
     (dict(num_pages=1 << 31), UNSUP), (dict(batch=5000), UNSUP),
-    (dict(max_pages=1 << 25, table_stride=1 << 25), UNSUP),
+    (dict(max_pages=1 << 24, table_stride=1 << 24), UNSUP),
 ]
 ROWS = [
     (dict(lengths=0), BAD), (dict(lengths=18), UNSUP), (dict(k=0), BAD), (dict(v=0), BAD),

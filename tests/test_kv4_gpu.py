@@ -396,6 +396,14 @@ def test_bad_pages_and_lengths_are_reported_and_skipped():
     assert device_status() == _lib.DEVICE_STATUS_KV4_BAD_PAGE
     assert torch.equal(cache.pages, before)
     reset_device_status()
+    kv4_append(cache, x, x, table, ints([-2, -1000]))  # would reach slots 0 and 1
+    assert device_status() == _lib.DEVICE_STATUS_KV4_BAD_LENGTH
+    assert torch.equal(cache.pages, before)
+    reset_device_status()
+    kv4_append(cache, x, x, table, ints([3, 4]), counts=ints([-1, 0]))
+    assert device_status() == _lib.DEVICE_STATUS_KV4_BAD_LENGTH
+    assert torch.equal(cache.pages, before)
+    reset_device_status()
     k, v = kv4_expand(cache, bad, ints([62, 46]), 4)
     assert device_status() == _lib.DEVICE_STATUS_KV4_BAD_PAGE
     assert (k[0, 2:] == 0).all() and (v[1, 2:] == 0).all() and (k[0, :2] != 0).any()
@@ -649,6 +657,7 @@ def test_python_surface_refuses():
             lambda: kv4_attention(q, cache, table, n, decay=math.nan),
             lambda: kv4_attention(q, cache, table, n, softmax_scale=0.0),
             lambda: kv4_attention(q, cache, table, n, out=q.half()),
+            lambda: kv4_attention(q, cache, table, n, out=q),
             lambda: kv4_attention(q[:, :1].expand(2, 3, 4, 128), cache, table, n),
             lambda: kv4_append(cache, x, x.half(), table, n),
             lambda: kv4_append(cache, x, q, table, n),
