@@ -1,5 +1,4 @@
-// Attention of a few new queries over the 4-bit cache: one pass over the
-// cache, memory-bound up to some 16 query rows a key head.
+// Attention of a few new queries over the 4-bit cache, in one pass over it.
 //
 // For a key head the rows are its new tokens x query heads, in tiles of 8 NT.
 // A warp takes 32 tokens at a time:
@@ -11,8 +10,18 @@
 //
 // so scales touch the few scores, never the 128 channels, and the rows, not
 // the tokens, are the narrow side of the instruction. tcgen05 would pad the
-// rows to 64 or more, and its operands would have to be written out to shared
-// memory in 16 bits first, four times the bytes that arrive.
+// rows to 64 or more and take the codes from shared memory in 16 bits, four
+// times the bytes that arrive; e4m3, whose first 16 numbers are evenly spaced
+// and so hold a code in a byte, is emulated by two fp16 products in mma.sync.
+//
+// What bounds it is not the memory but the instructions that make operands of
+// codes: of some 780 a tile (8 rows, groups of 64) 280 belong to the values,
+// 220 to the keys, 130 to the copies. The matrix pipe is a fifth busy and can
+// be left out without a change in time, the ALU half. Measured: 32 sequences of
+// 3.3k to 8.2k tokens, 8 heads, 8 rows: 63 us, 3.4 TB/s; one of 131,071 tokens,
+// 8 heads, 4 rows, groups of 32: 52 us, 3.2 TB/s; without any arithmetic the
+// copies alone take 44 and 35 us. 12 warps on an SM have the 168 registers that
+// a tile needs; 16 with 128 spill (groups of 32: 100 us), 8 are 10 % slower.
 //
 // Codes become fp16 integers by one LOP3 and one HFMA2 a pair: a nibble u in
 // bits 0-3 of a half, or'ed with 0x6400, is 1024 + u, in bits 4-7 it is 1024 +
