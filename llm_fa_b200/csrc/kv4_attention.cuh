@@ -290,15 +290,16 @@ struct Kv4Ring {
     put = put + 1 == STAGES ? 0 : put + 1;
   }
   // Waits for the next tile, at most timeout_ns; false when its copies did not arrive (or were
-  // not issued, after an earlier one did not).
+  // not issued, after an earlier one did not). All lanes get the same answer: what follows is
+  // the whole warp's.
   __device__ __forceinline__ bool wait(unsigned long long timeout_ns) {
     if (pending == 0) return false;
     const uint32_t bar = bars + take * 8;
-    if (ptx::mbar_try_wait(bar, parity)) return true;
+    if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
     const uint64_t t0 = ptx::globaltimer_ns();
     for (uint32_t it = 1;; ++it) {
-      if (ptx::mbar_try_wait(bar, parity)) return true;
-      if ((it & 63u) == 0 && ptx::globaltimer_ns() - t0 > timeout_ns) return false;
+      if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+      if ((it & 63u) == 0 && __any_sync(0xffffffffu, ptx::globaltimer_ns() - t0 > timeout_ns)) return false;
     }
   }
   __device__ __forceinline__ uint32_t tile() const { return base + take * kTileBytes; }
