@@ -352,7 +352,9 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
   if ((rc = check_cache(cache, seqs, true, &p.pool, &p.seqs)) != LLMFA_OK) return rc;
   if ((rc = check_tokens(tokens, dtype, counts)) != LLMFA_OK) return rc;
   if (heads_q < 1 || heads_q % cache->heads != 0) return LLMFA_ERR_INVALID_ARGUMENT;
-  if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return LLMFA_ERR_INVALID_ARGUMENT;
+  // it is used times log2(e), which has to stay in fp32's range too
+  const float scale_log2 = softmax_scale * 1.4426950408889634f;
+  if (!(softmax_scale > 0.f) || !std::isfinite(scale_log2)) return LLMFA_ERR_INVALID_ARGUMENT;
   if (decay != decay || decay > 1.f) return LLMFA_ERR_INVALID_ARGUMENT;
   if ((rc = check_rows(q, q_strides, seqs->batch, tokens, heads_q, &p.q)) != LLMFA_OK) return rc;
   if ((rc = check_rows(o, o_strides, seqs->batch, tokens, heads_q, &p.o)) != LLMFA_OK) return rc;
@@ -390,7 +392,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
   p.group = static_cast<int>(heads_q / cache->heads);
   p.row_tiles = shape.row_tiles;
   p.page_stride = static_cast<uint64_t>(kv4_block_offset(p.pool, 1, 0, 0));
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   p.decay = decay;
   p.timeout_ns = wait_limit_ns();
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

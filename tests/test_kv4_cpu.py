@@ -160,6 +160,12 @@ def test_attention_refuses_without_cuda(L, kw, code):
     assert _attend(L, **kw) == code
 
 
+@pytest.mark.parametrize("scale,code", [(3e38, BAD), (2.4e38, BAD), (-1.0, BAD)])
+def test_attention_refuses_a_scale_that_log2_e_takes_out_of_range(L, scale, code):
+    assert 2.4e38 * 1.4427 > 3.4029e38
+    assert _attend(L, scale=scale) == code
+
+
 def _select(L, **kw):
     c, s, kw = _structs(kw)
     g = lambda n, d: kw.get(n, d)  # noqa: E731
