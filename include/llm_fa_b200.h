@@ -301,7 +301,8 @@ int llmfa_kv4_evict_workspace_size(int64_t batch, int64_t heads, int64_t keep, u
  * recent), go after all others. The freed slots below keep take, in ascending
  * order, the surviving tokens at or above it: src[b][head][d] is the slot
  * whose token slot d is to hold, -1 past the new length min(lengths[b], keep),
- * which new_lengths[b] receives (it must not be seqs->lengths itself).
+ * which new_lengths[b] receives (it must not be seqs->lengths itself). Tables
+ * of more than about 14 million slots are LLMFA_ERR_UNSUPPORTED.
  */
 int llmfa_kv4_evict_select(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs,
                            const int32_t* seen, int64_t keep, int64_t recent, int32_t* src,

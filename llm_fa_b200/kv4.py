@@ -241,7 +241,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
 
     decay (0 to 1) also tracks the weight that each token received: cache.weights becomes
     decay * cache.weights + the softmax weights of this call, summed over the new tokens and the
-    query heads that share a key head. 1.0 accumulates; 0.0 stores this call's sums alone.
+    query heads that share a key head. 1.0 accumulates; 0.0 stores this call's sums alone. The
+    sequences of such a call share no pages: their sums would overwrite one another.
 
     softmax_scale defaults to 1/sqrt(128). With return_lse, returns (O, lse): the natural-log
     log-sum-exp of every row, fp32 [batch, heads_q, tokens].
