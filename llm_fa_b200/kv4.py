@@ -213,14 +213,15 @@ def kv4_expand(cache: KV4Cache, page_table: torch.Tensor, start: torch.Tensor, t
         if dtype not in _DTYPES or tokens < 1:
             raise RuntimeError("kv4_expand needs tokens >= 1 and bfloat16 or float16, got "
                                f"{tokens}, {dtype}")
-        shape = (B, tokens, cache._heads, HEAD_DIM)
-        out = (torch.empty(shape, dtype=dtype, device=cache._device),
-               torch.empty(shape, dtype=dtype, device=cache._device))
-    k, v = out
-    shape, ks = _rows(k, "k", cache, B, cache._heads)
-    _, vs = _rows(v, "v", cache, B, cache._heads, like=k)
-    if shape[1] != tokens:
-        raise RuntimeError(f"out holds {shape[1]} tokens, expected {tokens}")
+        k = torch.empty(B, tokens, cache._heads, HEAD_DIM, dtype=dtype, device=cache._device)
+        v = torch.empty_like(k)
+        ks = vs = _strides3(k.stride())
+    else:
+        k, v = out
+        shape, ks = _rows(k, "k", cache, B, cache._heads)
+        _, vs = _rows(v, "v", cache, B, cache._heads, like=k)
+        if shape[1] != tokens:
+            raise RuntimeError(f"out holds {shape[1]} tokens, expected {tokens}")
     _call(cache, "llmfa_kv4_expand", seqs, k.data_ptr(), ks, v.data_ptr(), vs,
           None if counts is None else _ints(counts, "counts", cache, B), tokens, _DTYPES[k.dtype])
     return k, v
