@@ -78,7 +78,7 @@ constexpr float kKv4Slack = 6.f;
 constexpr int kKv4WeightBits = 8;  // w < 2^(kKv4WeightBits + kKv4Slack)
 constexpr int kStatusTimeout = 0x1000;  // + wait site: a bounded wait gave up
 constexpr int kSiteKv4Tile = 13;
-constexpr unsigned long long kKv4DrainNs = 1000000;
+constexpr unsigned long long kKv4DrainNs = 1000000;  // for copies in flight after that
 
 // ---------------------------------------------------------------- instructions
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -104,6 +104,9 @@ __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
+}
+__device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 // A token's NG pairs.
 template <int NG>
@@ -177,15 +180,15 @@ __device__ __forceinline__ Kv4Row kv4_row(const Kv4AttnParams& p, int h, int c, 
 // The query rows of a segment, as a lane's B fragments: of n-tile nt, lane (g,
 // c) has of row g the channels 32 j + 8 c .. + 7, the codes of its word j. Step
 // 2j takes nibbles 0, 4 and 1, 5, step 2j + 1 nibbles 2, 6 and 3, 7. Of rows
-// 2c, 2c + 1, whose scores the lane gets, it has the factor and the limit.
+// 2c, 2c + 1, whose scores the lane gets, it has the factor.
 template <int NT>
 struct Kv4Queries {
   static constexpr bool kInRegisters = NT <= 2;  // else in the warp's shared memory
   uint2 frag[8][kInRegisters ? NT : 1];
   uint2* shared;  // [8][NT][32]
   float factor[NT][2];
-  int limit[NT][2];  // slots that the row sees
-  int all;           // slots that every live row sees
+  uint32_t limits;  // shared address: slots that each row sees; only tiles at a border read them
+  int all;          // slots that every live row sees
 
   __device__ __forceinline__ uint2 operator()(int step, int nt) const {
     if constexpr (kInRegisters) return frag[step][nt];
@@ -213,7 +216,11 @@ struct Kv4Queries {
   __device__ __forceinline__ void set(const Kv4AttnParams& p, int h, int r0, int n, int c,
                                       const uint4 (&raw)[NT][4]) {
     const int lane = threadIdx.x & 31, cc = lane & 3;
-    if constexpr (!kInRegisters) __syncwarp();  // the last segment's are read
+    __syncwarp();  // the last segment's are read
+    for (int r = lane; r < 8 * NT; r += 32) {
+      const Kv4Row row = kv4_row(p, h, c, r0 + r);
+      st_shared_u32(limits + 4 * r, row.live ? kv4_visible(n, c, row.i, p.causal) : 0);
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float x[4][8], top = 0.f, bad = 0.f;
@@ -256,18 +263,22 @@ struct Kv4Queries {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         factor[nt][k] = __shfl_sync(0xffffffffu, f, (2 * cc + k) * 4);
-        const Kv4Row row = kv4_row(p, h, c, r0 + 8 * nt + 2 * cc + k);
-        limit[nt][k] = row.live ? kv4_visible(n, c, row.i, p.causal) : 0;
       }
     }
     all = p.causal ? kv4_visible(n, c, r0 / p.group, true) : n;
-    if constexpr (!kInRegisters) __syncwarp();
+    __syncwarp();
+  }
+  // Of rows 2c, 2c + 1 of n-tile nt.
+  __device__ __forceinline__ int2 limit(int nt) const {
+    const uint2 v = ld_shared_v2(limits + (8 * nt + 2 * (threadIdx.x & 3)) * 4);
+    return make_int2(v.x, v.y);
   }
 };
 
 // ---------------------------------------------------------------- tiles
 // A warp's ring of tiles: STAGES buffers of kKv4TokenBlocks blocks, each of
-// which holds `BYTES` from the block's start (all of it, or the keys' half).
+// which holds `BYTES` from the block's start (all of it, or the keys' half). A
+// barrier each, and behind these two flags: a wait ran out, a page is missing.
 template <int STAGES, int BYTES>
 struct Kv4Ring {
   static constexpr int kTileBytes = kKv4TokenBlocks * BYTES;
@@ -289,18 +300,28 @@ struct Kv4Ring {
     ++pending;
     put = put + 1 == STAGES ? 0 : put + 1;
   }
-  // Waits for the next tile, at most timeout_ns; false when its copies did not arrive (or were
-  // not issued, after an earlier one did not). All lanes get the same answer: what follows is
-  // the whole warp's.
-  __device__ __forceinline__ bool wait(unsigned long long timeout_ns) {
-    if (pending == 0) return false;
+  // Waits for the next tile, at most timeout_ns. A lane that gives up sets the warp's flag and goes
+  // on with what the buffer holds: the lanes must not part here, as what follows is the whole
+  // warp's. Past the next __syncwarp all see the flag, and issue no more; the end reports it.
+  __device__ __forceinline__ void wait(unsigned long long timeout_ns) {
+    if (pending == 0) return;
     const uint32_t bar = bars + take * 8;
-    if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+    if (ptx::mbar_try_wait(bar, parity)) return;
     const uint64_t t0 = ptx::globaltimer_ns();
+    const unsigned long long limit_ns = failed() ? kKv4DrainNs : timeout_ns;
     for (uint32_t it = 1;; ++it) {
-      if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
-      if ((it & 63u) == 0 && __any_sync(0xffffffffu, ptx::globaltimer_ns() - t0 > timeout_ns)) return false;
+      if (ptx::mbar_try_wait(bar, parity)) return;
+      if ((it & 63u) == 0 && ptx::globaltimer_ns() - t0 > limit_ns) break;
     }
+    st_shared_u32(bars + STAGES * 8, 1);
+  }
+  __device__ __forceinline__ bool failed() const { return ld_shared_u32(bars + STAGES * 8) != 0; }
+  __device__ __forceinline__ void no_page() const { st_shared_u32(bars + STAGES * 8 + 4, 1); }
+  // At the warp's end: atomics at the tiles would cost registers there.
+  __device__ __forceinline__ void report(const Kv4Seqs& seqs) const {
+    __syncwarp();
+    if (ld_shared_u32(bars + STAGES * 8 + 4) != 0) kv4_report(seqs, kStatusKv4BadPage);
+    if (failed()) kv4_report(seqs, kStatusTimeout + kSiteKv4Tile);
   }
   __device__ __forceinline__ uint32_t tile() const { return base + take * kTileBytes; }
   __device__ __forceinline__ uint32_t blocks() const { return have & 3u; }
@@ -344,27 +365,33 @@ struct Kv4Loader {
     table = p.seqs.table + s.b * p.seqs.table_stride;
     pages = p.pool.pages + kv4_block_offset(p.pool, 0, s.i / row_tiles, 0);
   }
-  __device__ __forceinline__ void find(const Kv4AttnParams& p) {
+  template <typename Ring>
+  __device__ __forceinline__ void find(const Kv4AttnParams& p, const Ring& ring) {
     page = -1;
     if (slot < n) {  // n is inside the table
       page = table[slot >> p.pool.page_shift];
       if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.pool.num_pages)) {
         page = -1;
-        kv4_report(p.seqs, kStatusKv4BadPage);
+        ring.no_page();
       }
     }
   }
-  __device__ __forceinline__ void start(const Kv4AttnParams& p, const Kv4Plan& plan,
+  template <typename Ring>
+  __device__ __forceinline__ void start(const Kv4AttnParams& p, const Kv4Plan& plan, const Ring& ring,
                                         const Kv4Segment& s, bool any, int row_tiles) {
     more = any;
     if (!more) return;
     enter(p, plan, s, row_tiles);
-    find(p);
+    find(p, ring);
   }
   template <int NG, typename Ring>
   __device__ __forceinline__ void issue(const Kv4AttnParams& p, const Kv4Plan& plan, Ring& ring,
                                         int row_tiles) {
     if (!more) return;
+    if (ring.failed()) {
+      more = false;
+      return;
+    }
     const int block = (slot & ((1 << p.pool.page_shift) - 1)) >> 4;
     ring.issue(pages + static_cast<uint64_t>(page) * p.page_stride + block * kv4_block_bytes(NG),
                page >= 0);
@@ -376,7 +403,7 @@ struct Kv4Loader {
       if (!more) return;
       enter(p, plan, s, row_tiles);
     }
-    find(p);
+    find(p, ring);
   }
 };
 
@@ -515,12 +542,14 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
           for (int grp = 0; grp < NG; ++grp) pv[s][u][grp] = 0;
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          const int2 limit = q.limit(nt);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            if (here && slot < q.limit[nt][k]) seen |= 1u << (((2 * s + u) * NT + nt) * 2 + k);
+            if (here && slot < (k == 0 ? limit.x : limit.y)) seen |= 1u << (((2 * s + u) * NT + nt) * 2 + k);
             else x[s][nt][2 * u + k] = -INFINITY;
           }
+        }
       }
     }
   }
@@ -715,7 +744,8 @@ struct Kv4AttnSmem {
   uint2 q[Kv4Queries<NT>::kInRegisters ? 1 : WARPS][8 * NT * 32];
   Kv4Plan plan;
   Kv4Segment seg[WARPS];
-  uint64_t bar[WARPS][STAGES];
+  uint64_t bar[WARPS][STAGES + 1];  // and the ring's flags
+  uint2 limit[WARPS][4 * NT];
 };
 
 template <typename T, int NT, int NG, int WARPS, int STAGES, int CTAS>
@@ -729,6 +759,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
 
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) ptx::mbar_init(ptx::smem_u32(&sm.bar[warp][s]), 1);
+    sm.bar[warp][STAGES] = 0;
     ptx::fence_mbar_init();
   }
   kv4_make_plan<kThreads>(p, p.pool.heads * p.row_tiles,
@@ -743,6 +774,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
                                             ptx::smem_u32(sm.bar[warp])};
   Kv4Queries<NT> q;
   q.shared = sm.q[Kv4Queries<NT>::kInRegisters ? 0 : warp];
+  q.limits = ptx::smem_u32(sm.limit[warp]);
   uint4 raw[NT][4];
   auto fetch = [&] {
     const int h = seg.i / p.row_tiles;
@@ -754,12 +786,11 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   if (kEarly) fetch();
   Kv4Loader loader;
   loader.seg = &sm.seg[warp];
-  loader.start(p, plan, seg, more, p.row_tiles);
+  loader.start(p, plan, ring, seg, more, p.row_tiles);
   for (int s = 0; s < STAGES; ++s) loader.template issue<NG>(p, plan, ring, p.row_tiles);
 
   // rows g and g + 8 of the keys' operand are tokens tok and tok + 8 of a block
   const int tok = (g >> 1) + 4 * (g & 1);
-  unsigned long long limit_ns = p.timeout_ns;
   while (more) {
     const int h = seg.i / p.row_tiles, r0 = (seg.i - h * p.row_tiles) * kRows;
     const int n = plan.held[seg.b], c = plan.news[seg.b];
@@ -786,14 +817,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
                     : p.scores + (static_cast<long long>(seg.b) * p.pool.heads + h) *
                                      kv4_capacity(p.pool, p.seqs) * rows;
     for (int t = seg.lo; t < seg.hi; ++t) {
-      uint32_t blocks = ring.blocks();
-      if (!ring.wait(limit_ns)) {
-        // The copies never came: report, issue no more, give those in flight a moment each.
-        kv4_report(p.seqs, kStatusTimeout + kSiteKv4Tile);
-        limit_ns = kKv4DrainNs;
-        loader.more = false;
-        blocks = 0;
-      }
+      const uint32_t blocks = ring.blocks();
+      ring.wait(p.timeout_ns);
       const int slot0 = t * kKv4TileTokens;
       if (slot0 + kKv4TileTokens > q.all || blocks != 3u)
         kv4_tile<T, NT, NG, true>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
@@ -838,6 +863,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
     more = seg.next(plan.split);
     if (kEarly && more) fetch();
   }
+  ring.report(p.seqs);
 }
 
 // Joins the pieces of the units that were cut: one block a unit and row; a
@@ -933,7 +959,8 @@ struct Kv4WeightsSmem {
   int page[WARPS][STAGES][kKv4TokenBlocks];
   Kv4Plan plan;
   Kv4Segment seg[WARPS];
-  uint64_t bar[WARPS][STAGES];
+  uint64_t bar[WARPS][STAGES + 1];  // and the ring's flags
+  uint2 limit[WARPS][4 * NT];
 };
 
 template <typename T, int NT, int NG, int WARPS, int STAGES, int CTAS>
@@ -946,6 +973,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) ptx::mbar_init(ptx::smem_u32(&sm.bar[warp][s]), 1);
+    sm.bar[warp][STAGES] = 0;
     ptx::fence_mbar_init();
   }
   kv4_make_plan<kThreads>(p, p.pool.heads, reinterpret_cast<uint32_t*>(smem_raw + sizeof(Smem)),
@@ -957,7 +985,6 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
                                            ptx::smem_u32(sm.bar[warp])};
   Kv4Loader loader{};
   loader.seg = &sm.seg[warp];
-  unsigned long long limit_ns = p.timeout_ns;
   auto issue = [&] {
     if (loader.more && lane < kKv4TokenBlocks) sm.page[warp][ring.put][lane] = loader.page;
     loader.template issue<NG>(p, plan, ring, 1);
@@ -965,8 +992,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   const int tok = (g >> 1) + 4 * (g & 1);
   Kv4Queries<NT> q;
   q.shared = sm.q[Kv4Queries<NT>::kInRegisters ? 0 : warp];
+  q.limits = ptx::smem_u32(sm.limit[warp]);
   for (int rt = 0; rt < p.row_tiles; ++rt) {
-    loader.start(p, plan, first, limit_ns == p.timeout_ns, 1);  // no more after a timeout
+    loader.start(p, plan, ring, first, !ring.failed(), 1);  // no more after a timeout
     for (int s = 0; s < STAGES; ++s) issue();
     if (rt == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows' log-sum-exp
     Kv4Segment seg = first;
@@ -985,13 +1013,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
                                 : INFINITY;
         }
       for (int t = seg.lo; t < seg.hi; ++t) {
-        uint32_t blocks = ring.blocks();
-        if (!ring.wait(limit_ns)) {
-          kv4_report(p.seqs, kStatusTimeout + kSiteKv4Tile);
-          limit_ns = kKv4DrainNs;
-          loader.more = false;
-          blocks = 0;
-        }
+        const uint32_t blocks = ring.blocks();
+        ring.wait(p.timeout_ns);
         const uint32_t tile = ring.tile();
         const int slot0 = t * kKv4TileTokens;
         float sum[4];
@@ -1004,12 +1027,14 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
             const int slot = slot0 + 16 * s + tok + 8 * u;
             float w = 0.f;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+              const int2 limit = q.limit(nt);
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 const float pr = ptx::ex2_mufu(fmaf(x[nt][2 * u + k], q.factor[nt][k], -lse[nt][k]));
-                w += slot < q.limit[nt][k] ? pr : 0.f;
+                w += slot < (k == 0 ? limit.x : limit.y) ? pr : 0.f;
               }
+            }
             sum[2 * s + u] = w;
           }
         }
@@ -1021,7 +1046,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
         // lane cc of a quad stores token cc of its four
         const float mine = cc == 0 ? sum[0] : cc == 1 ? sum[1] : cc == 2 ? sum[2] : sum[3];
         const int s = cc >> 1, slot = slot0 + 16 * s + tok + 8 * (cc & 1);
-        if (((blocks >> s) & 1u) != 0 && slot < n) {
+        if (((blocks >> s) & 1u) != 0 && slot < n && !ring.failed()) {
           const int page = sm.page[warp][ring.take][s];
           float* w = p.pool.weights + kv4_token_index(p.pool, page, h, slot);
           *w = rt > 0 ? *w + mine : p.decay == 0.f ? mine : fmaf(p.decay, *w, mine);
@@ -1031,6 +1056,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
       }
     }
   }
+  ring.report(p.seqs);
 }
 
 }  // namespace llmfa
