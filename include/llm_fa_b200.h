@@ -264,6 +264,10 @@ int llmfa_kv4_expand(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, v
                      const int64_t k_strides[3], void* v, const int64_t v_strides[3],
                      const int32_t* counts, int64_t tokens, int dtype, void* stream);
 
+/* What llmfa_kv4_attention does with rows past a count, added up (0: leaves them as they were). */
+#define LLMFA_KV4_FILL_OUT 1 /* zeros in o */
+#define LLMFA_KV4_FILL_LSE 2 /* -inf in lse */
+
 /* Workspace of llmfa_kv4_attention, 16-byte aligned; capacity is max_pages *
  * page_size of a call that tracks, else 0. Its contents are not read across
  * calls; calls that share one must not overlap. */
@@ -277,7 +281,7 @@ int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t hea
  * i / (heads_q / heads); o may not alias q. seqs->lengths counts the new tokens, whose keys are
  * appended already. With causal != 0, new token i sees slots 0 .. lengths[b] -
  * counts[b] + i, else all. A row that sees no slot gets zeros (and lse -inf);
- * rows past a count are left as they were. lse as for llmfa_forward_lse, or
+ * rows past a count get what `fill` says. lse as for llmfa_forward_lse, or
  * NULL. decay >= 0 (at most 1) tracks: weights[slot] = decay * weights[slot] +
  * the slot's softmax weights summed over the new tokens and the query heads of
  * its head; with decay 0 the old value is not read. decay < 0 leaves weights
@@ -287,7 +291,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
                         const int64_t q_strides[3], void* o, const int64_t o_strides[3],
                         float* lse, const int64_t lse_strides[2], const int32_t* counts,
                         int64_t heads_q, int64_t tokens, int causal, float softmax_scale,
-                        float decay, int dtype, void* workspace, uint64_t workspace_bytes,
+                        float decay, int fill, int dtype, void* workspace, uint64_t workspace_bytes,
                         void* stream);
 
 /* Workspace of llmfa_kv4_evict_select, 16-byte aligned. */

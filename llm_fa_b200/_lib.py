@@ -26,12 +26,13 @@ DEVICE_STATUS_KV4_BAD_LENGTH = 0x2002
 DEVICE_STATUS_KV4_BAD_SOURCE = 0x2003
 LLMFA_BF16 = 0
 LLMFA_FP16 = 1
+LLMFA_KV4_FILL_OUT = 1
+LLMFA_KV4_FILL_LSE = 2
 
 _I64x3 = ctypes.c_int64 * 3
 _I64x2 = ctypes.c_int64 * 2
 _lock = threading.Lock()
 _lib = None
-
 
 
 class Kv4Cache(ctypes.Structure):
@@ -100,7 +101,7 @@ SIGNATURES = {
     "llmfa_kv4_attention": (ctypes.c_int, _KV4 + [
         ctypes.c_void_p, _I64x3, ctypes.c_void_p, _I64x3, ctypes.c_void_p,
         ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
-        ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_int, ctypes.c_void_p,
+        ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
         ctypes.c_uint64, ctypes.c_void_p]),
     "llmfa_kv4_evict_workspace_size": (ctypes.c_int, [
         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_uint64)]),

@@ -345,8 +345,8 @@ int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t hea
 int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, const void* q,
                         const int64_t q_strides[3], void* o, const int64_t o_strides[3], float* lse,
                         const int64_t lse_strides[2], const int32_t* counts, int64_t heads_q,
-                        int64_t tokens, int causal, float softmax_scale, float decay, int dtype,
-                        void* workspace, uint64_t workspace_bytes, void* stream) {
+                        int64_t tokens, int causal, float softmax_scale, float decay, int fill,
+                        int dtype, void* workspace, uint64_t workspace_bytes, void* stream) {
   Kv4AttnParams p{};
   int rc;
   if ((rc = check_cache(cache, seqs, true, &p.pool, &p.seqs)) != LLMFA_OK) return rc;
@@ -356,6 +356,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
   const float scale_log2 = softmax_scale * 1.4426950408889634f;
   if (!(softmax_scale > 0.f) || !std::isfinite(scale_log2)) return LLMFA_ERR_INVALID_ARGUMENT;
   if (decay != decay || decay > 1.f) return LLMFA_ERR_INVALID_ARGUMENT;
+  if ((fill & ~(LLMFA_KV4_FILL_OUT | LLMFA_KV4_FILL_LSE)) != 0) return LLMFA_ERR_INVALID_ARGUMENT;
   if ((rc = check_rows(q, q_strides, seqs->batch, tokens, heads_q, &p.q)) != LLMFA_OK) return rc;
   if ((rc = check_rows(o, o_strides, seqs->batch, tokens, heads_q, &p.o)) != LLMFA_OK) return rc;
   if (lse != nullptr) {
@@ -389,6 +390,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
   p.heads_q = static_cast<int>(heads_q);
   p.tokens = static_cast<int>(tokens);
   p.causal = causal != 0;
+  p.fill = fill;
   p.group = static_cast<int>(heads_q / cache->heads);
   p.row_tiles = shape.row_tiles;
   p.page_stride = static_cast<uint64_t>(kv4_block_offset(p.pool, 1, 0, 0));

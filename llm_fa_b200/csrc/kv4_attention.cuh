@@ -47,6 +47,7 @@
 #pragma once
 #include <type_traits>
 
+#include "../../include/llm_fa_b200.h"
 #include "kv4_plan.cuh"
 #include "kv4_quant.cuh"
 #include "ptx.cuh"
@@ -66,6 +67,7 @@ struct Kv4AttnParams {
   float* row_lse;   // [batch][tokens][heads_q], log2 units; null without tracking
   float* scores;    // [batch][heads][capacity][rows], log2 units; null where they are not kept
   int heads_q, tokens, causal;
+  int fill;  // LLMFA_KV4_FILL_*: what rows past a count get
   int group, row_tiles;
   uint64_t page_stride;  // bytes of a page, all heads
   float scale_log2;  // softmax_scale * log2(e)
@@ -704,20 +706,25 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
   }
 }
 
-// Channels `at` + 32 k .. + 3 of a finished row, and with channel 0 its log-sum-exp.
+// Channels `at` + 32 k .. + 3 of a finished row, and with channel 0 its log-sum-exp. A row past its
+// sequence's count is left alone or filled; what was summed for it means nothing.
 template <typename T, int K>
 __device__ __forceinline__ void kv4_write_row(const Kv4AttnParams& p, int b, int h, int c, int r,
                                               int at, const float4 (&f)[K], float m, float l) {
   const Kv4Row row = kv4_row(p, h, c, r);
-  if (!row.live) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* o = static_cast<T*>(p.o.ptr) + b * p.o.sb + row.i * p.o.st + row.hq * p.o.sh + at;
+  const int fill = row.i < p.tokens ? p.fill : 0;
+  if (row.live || (fill & LLMFA_KV4_FILL_OUT) != 0) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* o = static_cast<T*>(p.o.ptr) + b * p.o.sb + row.i * p.o.st + row.hq * p.o.sh + at;
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-    *reinterpret_cast<uint2*>(o + 32 * k) = make_uint2(Kv4Type<T>::pack(f[k].x * inv, f[k].y * inv),
-                                                       Kv4Type<T>::pack(f[k].z * inv, f[k].w * inv));
-  if (at == 0) {
-    const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+    for (int k = 0; k < K; ++k)
+      *reinterpret_cast<uint2*>(o + 32 * k) =
+          row.live ? make_uint2(Kv4Type<T>::pack(f[k].x * inv, f[k].y * inv),
+                                Kv4Type<T>::pack(f[k].z * inv, f[k].w * inv))
+                   : make_uint2(0, 0);
+  }
+  if (at == 0 && (row.live || (fill & LLMFA_KV4_FILL_LSE) != 0)) {
+    const float lse2 = !row.live || l == 0.f ? -INFINITY : m + log2f(l);
     if (p.lse != nullptr) p.lse[b * p.lse_sb + row.hq * p.lse_sh + row.i] = lse2 * 0.69314718055994531f;
     if (p.row_lse != nullptr)
       p.row_lse[(static_cast<long long>(b) * p.tokens + row.i) * p.heads_q + row.hq] = lse2;

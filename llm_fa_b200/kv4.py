@@ -259,10 +259,11 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
     elif not 0.0 <= decay <= 1.0:
         raise RuntimeError(f"decay must be between 0 and 1, got {decay}")
     n = None if counts is None else _ints(counts, "counts", cache, B)
+    fill = 0 if counts is None else _lib.LLMFA_KV4_FILL_LSE
     if out is None:
-        out = (torch.empty_like if counts is None else torch.zeros_like)(
-            q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os = _strides3(out.stride())
+        fill |= _lib.LLMFA_KV4_FILL_OUT
     else:
         _, os = _rows(out, "out", cache, B, Hq, like=q)
         if out.data_ptr() == q.data_ptr():
@@ -272,11 +273,12 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
     ws = torch.empty(nbytes, dtype=torch.uint8, device=cache._device)
     lse = ls = None
     if return_lse:
-        lse = torch.full((B, Hq, T), -math.inf, dtype=torch.float32, device=cache._device)
+        lse = torch.empty(B, Hq, T, dtype=torch.float32, device=cache._device)
         ls = _lib.strides2((Hq * T, T))
     _call(cache, "llmfa_kv4_attention", seqs, q.data_ptr(), qs, out.data_ptr(), os,
           lse.data_ptr() if return_lse else None, ls, n, Hq, T, bool(causal),
-          _SCALE if softmax_scale is None else float(softmax_scale), decay, _DTYPES[q.dtype],
+          _SCALE if softmax_scale is None else float(softmax_scale), decay, fill,
+          _DTYPES[q.dtype],
           ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
@@ -296,7 +298,7 @@ def kv4_evict_select(cache: KV4Cache, page_table: torch.Tensor, lengths: torch.T
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise RuntimeError(f"keep must be at least 1 and recent 0 to keep, got {keep}, {recent}")
-    src = torch.empty((B, cache._heads, keep), dtype=torch.int32, device=cache._device)
+    src = torch.empty(B, cache._heads, keep, dtype=torch.int32, device=cache._device)
     new = torch.empty(B, dtype=torch.int32, device=cache._device)
     nbytes = _size("llmfa_kv4_evict_workspace_size", B, cache._heads, keep)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=cache._device)

@@ -119,7 +119,7 @@ def _attend(L, **kw):
                                  _lib.strides2(g("ls", (64, 8))), _p(g("counts", 0)),
                                  g("heads_q", 2), g("tokens", 5), 1,
                                  ctypes.c_float(g("scale", 0.1)), ctypes.c_float(g("decay", -1.0)),
-                                 g("dtype", 0), _p(g("ws", 256)), g("ws_bytes", 1 << 30), None)
+                                 g("fill", 0), g("dtype", 0), _p(g("ws", 256)), g("ws_bytes", 1 << 30), None)
 
 
 SHARED = [
@@ -158,6 +158,11 @@ def test_expand_refuses_without_cuda(L, kw, code):
 ])
 def test_attention_refuses_without_cuda(L, kw, code):
     assert _attend(L, **kw) == code
+
+
+@pytest.mark.parametrize("fill", [4, -1, 8 | 1])
+def test_attention_refuses_unknown_fills(L, fill):
+    assert _attend(L, fill=fill) == BAD
 
 
 @pytest.mark.parametrize("scale,code", [(3e38, BAD), (2.4e38, BAD), (-1.0, BAD)])

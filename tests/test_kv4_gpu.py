@@ -574,6 +574,31 @@ def test_a_run_of_steps_with_eviction():
     assert device_status() == 0
 
 
+@pytest.mark.parametrize("lens,T,Hq,H,counts", [
+    ([40, 300, 0], 3, 8, 2, [1, 0, 0]),          # one piece a unit
+    ([5000, 4000], 40, 8, 2, [3, 40]),           # units cut; tiles without a row that is real
+    ([2000, 1, 33], 7, 32, 8, [0, 1, 7]),
+])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_past_a_count_in_memory_used_before(lens, T, Hq, H, counts, causal):
+    cache, table = filled(len(lens), H, lens, 64, 64, seed=3)
+    q = randn(len(lens), T, Hq, 128, seed=4)
+    for b, c in enumerate(counts):  # what padding holds is not for use
+        q[b, c:] = float("nan")
+    torch.use_deterministic_algorithms(True)  # new memory is filled with NaN
+    try:
+        assert torch.empty_like(q).isnan().all()
+        got = kv4_attention(q, cache, table, ints(lens), counts=ints(counts), causal=causal,
+                            return_lse=True)
+    finally:
+        torch.use_deterministic_algorithms(False)
+    assert device_status() == 0
+    for b, c in enumerate(counts):
+        assert (got[0][b, c:] == 0).all() and (got[1][b, :, c:] == -math.inf).all()
+    q.nan_to_num_(0.0)
+    check_attention(got, q, cache, table, lens, counts, causal=causal)
+
+
 def test_graph_capture_and_replay():
     B, H, Hq, n = 2, 2, 8, 500
     cache, table = filled(B, H, [n, n - 100], 64, 64, seed=1)
