@@ -16,8 +16,9 @@ namespace llmfa {
 
 constexpr int kKv4TileTokens = 32;
 constexpr int kKv4UnitCost = 1;
-// Least share: below two tiles a worker, joining costs more than waiting.
-constexpr int kKv4MinShare = 2 * (kKv4UnitCost + 1);
+// Least share: one tile. A tile takes a lone warp 1.2 us, more than joining its piece (1 x 1000
+// tokens, 8 heads: 12.4 us, with two tiles a worker 14.4, with three 16.4).
+constexpr int kKv4MinShare = kKv4UnitCost + 1;
 
 struct Kv4Split {
   const uint32_t* prefix;  // [batch + 1]: cost of one (head, row tile) of the sequences before b
