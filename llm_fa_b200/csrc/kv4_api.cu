@@ -203,23 +203,15 @@ int allow_smem(size_t bytes) {
   return LLMFA_OK;
 }
 
-int select_launch(const Kv4SelectParams& p, long long capacity, int sms, int32_t* movers,
-                  cudaStream_t st) {
-  const long long units = static_cast<long long>(p.seqs.batch) * p.pool.heads;
-  const int ctas = kv4_select_ctas(units, capacity, sms);
-  const int run = kv4_select_run(capacity, ctas);
-  const bool in_smem = kv4_select_in_smem(capacity);
-  const size_t smem = sizeof(Kv4SelectSmem) + static_cast<size_t>(run) / 8 +
-                      (in_smem ? static_cast<size_t>(run) * 4 : 0);
-  constexpr size_t kMost = 227 * 1024;
-  if (smem > kMost || units * ctas >= (1ll << 31)) return LLMFA_ERR_UNSUPPORTED;
-  int rc;
-  if ((rc = in_smem ? allow_smem<kv4_select_kernel<true>>(kMost)
-                    : allow_smem<kv4_select_kernel<false>>(kMost)) != LLMFA_OK)
-    return rc;
+template <bool SMEM, int WARPS>
+int select_launch_as(const Kv4SelectParams& p, unsigned grid, int ctas, size_t smem, size_t most,
+                     int32_t* movers, cudaStream_t st) {
+  constexpr auto kernel = kv4_select_kernel<SMEM, WARPS>;
+  const int rc = allow_smem<kernel>(most);
+  if (rc != LLMFA_OK) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(units * ctas));
-  cfg.blockDim = dim3(kKv4SelectThreads);
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(WARPS * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -227,12 +219,29 @@ int select_launch(const Kv4SelectParams& p, long long capacity, int sms, int32_t
   attr.val.clusterDim = {static_cast<unsigned>(ctas), 1, 1};
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, in_smem ? kv4_select_kernel<true> : kv4_select_kernel<false>, p, movers,
-                         ctas) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, p, movers, ctas) != cudaSuccess) {
     cudaGetLastError();
     return LLMFA_ERR_LAUNCH;
   }
   return LLMFA_OK;
+}
+
+int select_launch(const Kv4SelectParams& p, long long capacity, int sms, int32_t* movers,
+                  cudaStream_t st) {
+  const long long units = static_cast<long long>(p.seqs.batch) * p.pool.heads;
+  const int ctas = kv4_select_ctas(units, capacity, sms);
+  const bool in_smem = kv4_select_in_smem(capacity);
+  const int warps = in_smem ? kv4_select_warps(units, capacity, ctas, sms) : kKv4SelectMaxWarps;
+  const int run = kv4_select_run(capacity, ctas, warps);
+  const size_t smem = sizeof(Kv4SelectSmem) + static_cast<size_t>(run) / 8 +
+                      (in_smem ? static_cast<size_t>(run) * 4 : 0);
+  constexpr size_t kMost = 227 * 1024;
+  if (smem > kMost || units * ctas >= (1ll << 31)) return LLMFA_ERR_UNSUPPORTED;
+  const unsigned grid = static_cast<unsigned>(units * ctas);
+  if (!in_smem) return select_launch_as<false, kKv4SelectMaxWarps>(p, grid, ctas, smem, kMost, movers, st);
+  if (warps == 8) return select_launch_as<true, 8>(p, grid, ctas, smem, kMost, movers, st);
+  if (warps == 16) return select_launch_as<true, 16>(p, grid, ctas, smem, kMost, movers, st);
+  return select_launch_as<true, kKv4SelectMaxWarps>(p, grid, ctas, smem, kMost, movers, st);
 }
 
 template <typename T, int NT, int NG>

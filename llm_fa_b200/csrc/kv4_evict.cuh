@@ -21,7 +21,6 @@
 
 namespace llmfa {
 
-constexpr int kKv4SelectThreads = 1024;
 constexpr uint32_t kKv4Protected = 0xffffffffu;
 
 struct Kv4SelectParams {
@@ -74,28 +73,39 @@ __device__ __forceinline__ uint4 kv4_slot_keys(const Kv4SelectParams& p, const i
 //
 // Ranks are ballots within a row, sums over the rows of a warp, over the warps
 // of a CTA and over the CTAs of the cluster: six cluster barriers at most.
-constexpr int kKv4SelectWarps = kKv4SelectThreads / 32;
+constexpr int kKv4SelectMaxWarps = 32;
 constexpr int kKv4SelectMaxCluster = 8;
 constexpr int kKv4SelectKeys = 49152;  // keys that fit a CTA's shared memory (192 KB)
 constexpr int kKv4SelectBins = 256;
 
-constexpr int kKv4SelectRow = 4 * kKv4SelectThreads;  // a row for every warp
+// Slots of a row for each of a CTA's warps.
+__host__ __device__ constexpr int kv4_select_row(int warps) { return 4 * 32 * warps; }
 
 // Slots of one CTA's run: whole rows for whole warps.
-__host__ __device__ inline int kv4_select_run(long long n, int ctas) {
-  const long long all = static_cast<long long>(ctas) * kKv4SelectRow;
-  return static_cast<int>((n + all - 1) / all) * kKv4SelectRow;
+__host__ __device__ inline int kv4_select_run(long long n, int ctas, int warps) {
+  const long long all = static_cast<long long>(ctas) * kv4_select_row(warps);
+  return static_cast<int>((n + all - 1) / all) * kv4_select_row(warps);
 }
 
 // CTAs of a cluster; the keys of a run fit in shared memory where that is possible at all.
-// Doubled while a CTA has more than a row a warp and half the SMs would be idle.
+// Doubled while a CTA has more than 4096 slots and half the SMs would be idle.
 __host__ inline int kv4_select_ctas(long long units, long long capacity, int sms) {
   int ctas = 1;
   while (ctas < kKv4SelectMaxCluster &&
          (capacity > static_cast<long long>(ctas) * kKv4SelectKeys ||
-          (capacity > static_cast<long long>(ctas) * kKv4SelectRow && units * ctas * 2 <= 2 * sms)))
+          (capacity > static_cast<long long>(ctas) * 4096 && units * ctas * 2 <= 2 * sms)))
     ctas *= 2;
   return ctas;
+}
+// Warps of a CTA. Few for short runs, and where CTAs are many, as more of them are on an SM then
+// and their chains of barriers overlap; many where a CTA has an SM for itself and a long run.
+// Measured with 8, 16 and 32 warps, us: 8 x 1000 slots 8, 8, 10; 1664 x 239 24, 45, 88; 512 x 8192
+// 33, 37, 49; 64 x 8192 17, 14, 14; 64 x 32,768 29, 25, 33; 8 x 131,072 43, 31, 27; 256 x 32,768
+// (one CTA fits an SM) 130, 82, 61. 4 warps win 2 us on less than 256 slots and lose everywhere else.
+__host__ inline int kv4_select_warps(long long units, long long capacity, int ctas, int sms) {
+  const long long run = (capacity + ctas - 1) / ctas, blocks = units * ctas;
+  if (run <= 1024 || (run <= 8192 && blocks > 2 * sms)) return 8;
+  return run >= 16384 && (blocks <= sms || run > kKv4SelectKeys / 2) ? kKv4SelectMaxWarps : 16;
 }
 __host__ __device__ inline bool kv4_select_in_smem(long long capacity) {
   return capacity <= static_cast<long long>(kKv4SelectMaxCluster) * kKv4SelectKeys;
@@ -118,8 +128,8 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
 struct Kv4SelectSmem {
   alignas(16) uint32_t hist[4][kKv4SelectBins];
   uint32_t found[3];
-  uint32_t ties[kKv4SelectWarps];
-  uint32_t holes[kKv4SelectWarps], movers[kKv4SelectWarps];
+  uint32_t ties[kKv4SelectMaxWarps];
+  uint32_t holes[kKv4SelectMaxWarps], movers[kKv4SelectMaxWarps];
   uint32_t total[2];  // holes and movers of this CTA, for the cluster
 };
 
@@ -171,9 +181,10 @@ __device__ __forceinline__ void kv4_find_digit(const uint32_t* hist, int ctas, u
 }
 
 // Exclusive prefix over the warps of one value a warp, for lane 0's use by all its lanes.
+template <int WARPS>
 __device__ __forceinline__ uint32_t kv4_warps_before(const uint32_t* per_warp, uint32_t& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t v = per_warp[lane];
+  const uint32_t v = lane < WARPS ? per_warp[lane] : 0u;
   total = __reduce_add_sync(0xffffffffu, v);
   return __reduce_add_sync(0xffffffffu, lane < warp ? v : 0u);
 }
@@ -188,9 +199,10 @@ __device__ __forceinline__ uint32_t kv4_votes(const uint32_t (&vote)[4]) {
   return __popc(vote[0]) + __popc(vote[1]) + __popc(vote[2]) + __popc(vote[3]);
 }
 
-template <bool SMEM>
-__global__ void __launch_bounds__(kKv4SelectThreads)
+template <bool SMEM, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32)
     kv4_select_kernel(const __grid_constant__ Kv4SelectParams p, int32_t* movers, int ctas) {
+  constexpr int kThreads = WARPS * 32;
   extern __shared__ __align__(16) uint8_t select_smem[];
   Kv4SelectSmem& sm = *reinterpret_cast<Kv4SelectSmem*>(select_smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -200,7 +212,7 @@ __global__ void __launch_bounds__(kKv4SelectThreads)
   int32_t* src = p.src + static_cast<long long>(bh) * p.keep;
   if (h == 0 && rank == 0 && threadIdx.x == 0) p.new_lengths[b] = min(n, p.keep);
   if (go <= 0) {  // the whole cluster
-    for (int i = rank * kKv4SelectThreads + threadIdx.x; i < p.keep; i += ctas * kKv4SelectThreads)
+    for (int i = rank * kThreads + threadIdx.x; i < p.keep; i += ctas * kThreads)
       src[i] = i < n ? i : -1;
     return;
   }
@@ -209,8 +221,8 @@ __global__ void __launch_bounds__(kKv4SelectThreads)
   const long long border = static_cast<long long>(p.seen != nullptr ? p.seen[b] : n) - p.recent;
   const int first_recent = static_cast<int>(border < INT32_MIN ? INT32_MIN : border);
   const int32_t* table = p.seqs.table + b * p.seqs.table_stride;
-  const int run = kv4_select_run(n, ctas);
-  const int rows = run / kKv4SelectRow;  // of a warp; its rows are consecutive
+  const int run = kv4_select_run(n, ctas, WARPS);
+  const int rows = run / kv4_select_row(WARPS);  // of a warp; its rows are consecutive
   const int slot0 = rank * run + (warp * rows) * 128 + 4 * lane;
   uint32_t* masks = reinterpret_cast<uint32_t*>(select_smem + sizeof(Kv4SelectSmem)) + warp * rows * 4;
   uint4* keys = reinterpret_cast<uint4*>(select_smem + sizeof(Kv4SelectSmem) + run / 8) +
@@ -219,7 +231,7 @@ __global__ void __launch_bounds__(kKv4SelectThreads)
     return SMEM ? keys[r * 32] : kv4_slot_keys(p, table, h, slot0 + r * 128, n, first_recent);
   };
 
-  if (threadIdx.x < 4 * kKv4SelectBins) (&sm.hist[0][0])[threadIdx.x] = 0;
+  for (int i = threadIdx.x; i < 4 * kKv4SelectBins; i += kThreads) (&sm.hist[0][0])[i] = 0;
   __syncthreads();
 #pragma unroll 4
   for (int r = 0; r < rows; ++r) {
@@ -278,7 +290,7 @@ __global__ void __launch_bounds__(kKv4SelectThreads)
     if (lane == 0) sm.ties[warp] = mine;
     __syncthreads();
     uint32_t total;
-    equal += kv4_warps_before(sm.ties, total);
+    equal += kv4_warps_before<WARPS>(sm.ties, total);
   }
 
   uint32_t holes = 0, moves = 0;
@@ -316,7 +328,7 @@ __global__ void __launch_bounds__(kKv4SelectThreads)
   }
   __syncthreads();
   uint32_t all_holes, all_moves;
-  uint32_t hole = kv4_warps_before(sm.holes, all_holes), move = kv4_warps_before(sm.movers, all_moves);
+  uint32_t hole = kv4_warps_before<WARPS>(sm.holes, all_holes), move = kv4_warps_before<WARPS>(sm.movers, all_moves);
   if (threadIdx.x == 0) {
     sm.total[0] = all_holes;
     sm.total[1] = all_moves;

@@ -489,6 +489,32 @@ def test_select(kind, lens, keep, recent, page, H):
     assert device_status() == 0
 
 
+@pytest.mark.parametrize("kind", ["spread", "ties", "equal", "special"])
+@pytest.mark.parametrize("lens,keep,recent,page", [
+    ([239, 1, 0, 200, 100], 90, 20, 16),         # one row of slots a warp, or part of one
+    ([1025, 1024, 1023, 2049, 511], 700, 9, 64),
+    ([4096, 3000, 17, 4095, 2048], 2048, 64, 256),
+])
+def test_select_for_many_short_heads(kind, lens, keep, recent, page):
+    cache, table = pool(len(lens), 40, max(lens), page, 64, seed=5)
+    weights_like(cache, kind, seed=keep)
+    gen = torch.Generator().manual_seed(6)
+    cache.positions.copy_(torch.randint(0, 2 * max(lens), cache.positions.shape, generator=gen))
+    check_select(cache, table, lens, keep, recent, [2 * n for n in lens])
+    assert device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["spread", "ties"])
+@pytest.mark.parametrize("n,H", [(140_000, 1), (30_000, 160), (260_001, 2)])
+def test_select_long_runs(kind, n, H):
+    cache, table = pool(1, H, n, 256, 64, seed=2)
+    weights_like(cache, kind, seed=4)
+    gen = torch.Generator().manual_seed(7)
+    cache.positions.copy_(torch.randint(0, 2 * n, cache.positions.shape, generator=gen))
+    check_select(cache, table, [n - 3], n // 3, 100, [2 * n])
+    assert device_status() == 0
+
+
 @pytest.mark.parametrize("kind", ["spread", "ties", "special"])
 def test_select_from_a_table_too_long_for_shared_memory(kind):
     """A page table of 409,600 slots, of which 9000 are used."""
