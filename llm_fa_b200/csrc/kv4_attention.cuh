@@ -15,13 +15,16 @@
 // and so hold a code in a byte, is emulated by two fp16 products in mma.sync.
 //
 // What bounds it is not the memory but the instructions that make operands of
-// codes: of some 780 a tile (8 rows, groups of 64) 280 belong to the values,
-// 220 to the keys, 130 to the copies. The matrix pipe is a fifth busy and can
-// be left out without a change in time, the ALU half. Measured: 32 sequences of
-// 3.3k to 8.2k tokens, 8 heads, 8 rows: 63 us, 3.4 TB/s; one of 131,071 tokens,
-// 8 heads, 4 rows, groups of 32: 52 us, 3.2 TB/s; without any arithmetic the
-// copies alone take 44 and 35 us. 12 warps on an SM have the 168 registers that
-// a tile needs; 16 with 128 spill (groups of 32: 100 us), 8 are 10 % slower.
+// codes: of some 740 a tile (8 rows, groups of 64) 280 belong to the values,
+// 220 to the keys, 130 to the copies; 62 % of the issue slots are taken, by 12
+// warps on an SM that wait on one another's fixed latencies. The matrix pipe is
+// a fifth busy and can be left out without a change in time, the ALU half.
+// Measured: 32 sequences of 3.3k to 8.2k tokens, 8 heads, 8 rows: 64 us, 3.4
+// TB/s; one of 131,071 tokens, 8 heads, 4 rows, groups of 32: 53 us, 3.1 TB/s;
+// without any arithmetic the copies alone take 44 and 35 us, of which 12 are
+// launches, the plan and the first loads. 12 warps on an SM have the 168
+// registers that a tile needs; 14 with 144 and 16 with 128 spill (72 and 68 us,
+// groups of 32: 90 and 93), 8 are 10 % slower.
 //
 // Codes become fp16 integers by one LOP3 and one HFMA2 a pair: a nibble u in
 // bits 0-3 of a half, or'ed with 0x6400, is 1024 + u, in bits 4-7 it is 1024 +

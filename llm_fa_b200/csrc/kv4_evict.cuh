@@ -8,7 +8,7 @@
 // itself where nothing moves), -1 past the new length.
 //
 // Measured: 8 sequences of 8192 slots to 4096, 8 heads: 14 us; one of 131,072 to
-// 65,536: 29 us (1364 with one CTA a head). Both wait on the chain of passes, not
+// 65,536: 27 us (1364 with one CTA a head). Both wait on the chain of passes, not
 // on the 8 bytes a slot: cluster barriers take 1 us a digit.
 //
 // move: carries the tokens out. Sources lie at or above `keep` and targets

@@ -21,7 +21,7 @@
 // instructions: a thread takes 16 channels of the key and the value, so that
 // the addresses of a token's head are worked out by 8 threads; ranges are taken
 // on packed pairs; codes become numbers as fp16 integers. Measured: 8192 tokens
-// of 32 heads, groups of 32, in and back out: 37 + 34 us, 4.7 and 5.2 TB/s of
+// of 32 heads, groups of 32, in and back out: 38 + 31 us, 4.7 and 5.7 TB/s of
 // 6.6; with 8 channels a thread and 64-bit divisions in front it was 83 + 49.
 #pragma once
 #include <cuda_bf16.h>
