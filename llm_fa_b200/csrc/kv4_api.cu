@@ -92,7 +92,7 @@ int quant_grid(int64_t batch, int64_t tokens, int64_t heads, dim3* grid) {
 }
 
 // Rows of a key head, cut into tiles of 8 nt. A pass over the cache takes about 2, 3 and 4 parts of
-// time for 8, 16 and 24 rows (8 x 8192 tokens, 8 heads: 28, 35 and 46 us), which decides; tiles of
+// time for 8, 16 and 24 rows (8 x 8192 tokens, 8 heads: 31, 40 and 51 us), which decides; tiles of
 // 32 rows, at 81 us, spill registers and win nowhere.
 struct AttnShape {
   int64_t batch, heads, heads_q, tokens;

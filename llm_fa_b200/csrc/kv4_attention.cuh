@@ -19,26 +19,29 @@
 // 220 to the keys, 130 to the copies; 62 % of the issue slots are taken, by 12
 // warps on an SM that wait on one another's fixed latencies. The matrix pipe is
 // a fifth busy and can be left out without a change in time, the ALU half.
-// Measured: 32 sequences of 3.3k to 8.2k tokens, 8 heads, 8 rows: 64 us, 3.4
-// TB/s; one of 131,071 tokens, 8 heads, 4 rows, groups of 32: 53 us, 3.1 TB/s;
+// Measured: 32 sequences of 3.3k to 8.2k tokens, 8 heads, 8 rows: 72 us, 3.0
+// TB/s; one of 131,071 tokens, 8 heads, 4 rows, groups of 32: 59 us, 2.8 TB/s;
 // without any arithmetic the copies alone take 44 and 35 us, of which 12 are
 // launches, the plan and the first loads. 12 warps on an SM have the 168
 // registers that a tile needs; 14 with 144 and 16 with 128 spill (72 and 68 us,
 // groups of 32: 90 and 93), 8 are 10 % slower.
 //
-// Codes become fp16 integers by one LOP3 and one HFMA2 a pair: a nibble u in
+// Key codes become fp16 integers by one LOP3 and one HFMA2 a pair: a nibble u in
 // bits 0-3 of a half, or'ed with 0x6400, is 1024 + u, in bits 4-7 it is 1024 +
 // 16 u; taking off 1024 + zero (after a multiplication with 1/16 for the
 // latter: 64 + zero) leaves u - zero exactly. Its products with 11-bit numbers
-// are exact in fp32.
+// are exact in fp32. Value codes become bf16 integers in the same way, by 0x4300
+// (128 + u; the upper nibble is shifted down first, as bf16 has 7 bits).
 //
 // Roundings to 16 bits: q is scaled by a power of two per row so that its
 // largest element is near 2^13 (bf16 and fp16 values stay exact down to 2^-37
-// of it); w is fp16, 11 bits, scaled by a power of two per group so that the
-// largest value scale seen so far is in [1/2, 1): the running maximum of the
-// softmax, once more, for the scales. For fp16 outputs, whose own rounding is
-// no coarser, w's remainder is kept in a second fp16 and multiplied too. Sums,
-// maxima and outputs are fp32.
+// of it). w is the sum of two bf16 numbers, 2^-18 of it off: bf16 has fp32's
+// range, so that a token's value scale, whatever weight the token has, takes
+// nothing from the precision of another's. (One fp16 number with a common
+// exponent for the scales seen, 64 instead of 72 us for the batch below, loses
+// the values of tokens whose scales are 2^24 below that of a token of no weight.)
+// Sums, maxima and outputs are fp32; outputs are summed in units of 2^-24, so
+// that weights up to 2^kKv4Slack of many tokens do not pass fp32's range.
 //
 // The row maximum is lazy: p may reach 2^kKv4Slack before O is rescaled, so a
 // tile needs one vote instead of a reduction over lanes.
@@ -48,8 +51,6 @@
 // and values with their pairs) that a lane issues and the warp waits for, and
 // writes what it has of a unit. Warps of a block share nothing but the plan.
 #pragma once
-#include <type_traits>
-
 #include "../../include/llm_fa_b200.h"
 #include "kv4_plan.cuh"
 #include "kv4_quant.cuh"
@@ -80,7 +81,7 @@ struct Kv4AttnParams {
 
 constexpr int kKv4TokenBlocks = kKv4TileTokens / kKv4Block;  // blocks of a tile
 constexpr float kKv4Slack = 6.f;
-constexpr int kKv4WeightBits = 8;  // w < 2^(kKv4WeightBits + kKv4Slack)
+constexpr float kKv4Unit = 0x1p-24f;  // of values in sums
 constexpr int kStatusTimeout = 0x1000;  // + wait site: a bounded wait gave up
 constexpr int kSiteKv4Tile = 13;
 constexpr unsigned long long kKv4DrainNs = 1000000;  // for copies in flight after that
@@ -90,6 +91,14 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -168,6 +177,18 @@ __device__ __forceinline__ Kv4Zero kv4_zero(uint32_t pair_a, uint32_t pair_b) {
   z.lo = __byte_perm(a, b, 0x5410);
   z.hi = sub_f16x2(0x63806380u, z.lo);  // 960 - (1024 + zero)
   return z;
+}
+// Two codes less their zeros as bf16: 0x4300 + u is 128 + u, whose low nibble alone lies inside the
+// mantissa, and so for the zero, 128 + zero.
+__device__ __forceinline__ uint32_t kv4_value_pair(uint32_t w, uint32_t zero) {
+  uint32_t r, d;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(r) : "r"(w));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(r), "r"(zero));
+  return d;
+}
+__device__ __forceinline__ uint32_t kv4_value_zero(uint32_t pair_a, uint32_t pair_b) {
+  return __byte_perm(__float_as_uint(__uint_as_float(pair_a) + 8405760.f),
+                     __float_as_uint(__uint_as_float(pair_b) + 8405760.f), 0x5410);
 }
 __device__ __forceinline__ float kv4_scale(uint32_t pair) { return __uint_as_float(pair << 16); }
 
@@ -505,21 +526,19 @@ __device__ __forceinline__ void kv4_scores(uint32_t block, int tok, const Kv4Que
 }
 
 // A warp's running sums over the tokens of a segment.
-template <int NT, int NG>
+template <int NT>
 struct Kv4State {
   float o[8][NT][4];  // m-tile i: channels 32 (i / 2) + 4 g + 2 (i % 2) and + 1, rows 2c, 2c + 1
   float m[NT][2], l[NT][2];
-  int top[NG];        // exponent (biased) that the value scales seen so far stay within
 };
 
 // One tile of 32 tokens. RAGGED: some row does not see all of it (or a block is
 // missing): `blocks` says which are here, n what the sequence holds. `scores`,
 // if not null, takes the scores of rows r0 .. of the head's `rows`.
-template <typename T, int NT, int NG, bool RAGGED>
-__device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, int tok,
+template <int NT, int NG, bool RAGGED>
+__device__ __forceinline__ void kv4_tile(Kv4State<NT>& st, uint32_t tile, int tok,
                                          const Kv4Queries<NT>& q, uint32_t blocks, int slot0, int n,
                                          float* scores, int rows, int r0) {
-  constexpr bool kTwo = std::is_same<T, __half>::value;  // w in two halves
   constexpr int kBlockBytes = kv4_block_bytes(NG);
   const int lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   float x[2][NT][4];
@@ -577,15 +596,8 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
       }
   }
 
-  // maxima and value scales: a vote decides whether anything has to be rescaled
+  // maxima: a vote decides whether anything has to be rescaled
   bool grow = false;
-  float big[NG];
-#pragma unroll
-  for (int grp = 0; grp < NG; ++grp) {
-    big[grp] = fmaxf(fmaxf(kv4_scale(pv[0][0][grp]), kv4_scale(pv[0][1][grp])),
-                     fmaxf(kv4_scale(pv[1][0][grp]), kv4_scale(pv[1][1][grp])));
-    grow |= big[grp] >= __int_as_float((st.top[grp] + 1) << 23);
-  }
   float mx[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -595,16 +607,6 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
       grow |= mx[nt][k] > st.m[nt][k] + kKv4Slack;
     }
   if (__any_sync(0xffffffffu, grow)) {
-    float down[NG];
-#pragma unroll
-    for (int grp = 0; grp < NG; ++grp) {
-      // an infinite scale (exponent 255) is no scale of the format: it may overflow
-      const int e = max(st.top[grp],
-                        __reduce_max_sync(0xffffffffu, min(__float_as_int(big[grp]) >> 23, 254)));
-      const int shift = st.top[grp] - e;  // 2^shift, 0 below fp32's range
-      down[grp] = shift < -126 ? 0.f : __int_as_float((shift + 127) << 23);
-      st.top[grp] = e;
-    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -618,23 +620,21 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
         st.l[nt][k] *= a;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          st.o[i][nt][k] *= a * down[i * NG / 8];
-          st.o[i][nt][2 + k] *= a * down[i * NG / 8];
+          st.o[i][nt][k] *= a;
+          st.o[i][nt][2 + k] *= a;
         }
       }
   }
 
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    // p, and w = p * value scale * 2^(weight bits - top), as the product's B operand
-    uint32_t w[NG][NT][2], rest[kTwo ? NG : 1][NT][2];
+    // p, and w = p * value scale in two parts, as the product's B operand
+    uint32_t w[NG][NT][2], rest[NG][NT][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float f[NG];
 #pragma unroll
-      for (int grp = 0; grp < NG; ++grp)
-        f[grp] = kv4_scale(pv[s][u][grp]) *
-                 __int_as_float((127 + 127 + kKv4WeightBits - 1 - st.top[grp]) << 23);
+      for (int grp = 0; grp < NG; ++grp) f[grp] = kv4_scale(pv[s][u][grp]) * kKv4Unit;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float pr[2];
@@ -652,12 +652,10 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
         for (int grp = 0; grp < NG; ++grp) {
           // an unseen token may hold a NaN scale
           const float w0 = see[0] ? pr[0] * f[grp] : 0.f, w1 = see[1] ? pr[1] * f[grp] : 0.f;
-          const uint32_t h2 = Kv4Type<__half>::pack(w0, w1);
+          const uint32_t h2 = Kv4Type<__nv_bfloat16>::pack(w0, w1);
+          const float2 back = Kv4Type<__nv_bfloat16>::unpack(h2);
           w[grp][nt][u] = transpose8x8(h2);
-          if constexpr (kTwo) {
-            const float2 back = Kv4Type<__half>::unpack(h2);
-            rest[grp][nt][u] = transpose8x8(Kv4Type<__half>::pack(w0 - back.x, w1 - back.y));
-          }
+          rest[grp][nt][u] = transpose8x8(Kv4Type<__nv_bfloat16>::pack(w0 - back.x, w1 - back.y));
         }
       }
     }
@@ -665,7 +663,7 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
     // tokens c + 8, c + 12; a lane holds 16 channels of each, 4 of every 32.
     const uint32_t half = tile + s * kBlockBytes + kv4_half_bytes(NG);
     uint2 v[4];
-    Kv4Zero z[NG][2];
+    uint32_t z[NG][2];
     {
       uint32_t pz[4][NG];
 #pragma unroll
@@ -681,8 +679,8 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
       }
 #pragma unroll
       for (int grp = 0; grp < NG; ++grp) {
-        z[grp][0] = kv4_zero(pz[0][grp], pz[1][grp]);
-        z[grp][1] = kv4_zero(pz[2][grp], pz[3][grp]);
+        z[grp][0] = kv4_value_zero(pz[0][grp], pz[1][grp]);
+        z[grp][1] = kv4_value_zero(pz[2][grp], pz[3][grp]);
       }
     }
 #pragma unroll
@@ -693,23 +691,21 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT, NG>& st, uint32_t tile, in
       const uint32_t rb = k < 2 ? __byte_perm(v[2].x, v[3].x, sel) : __byte_perm(v[2].y, v[3].y, sel);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t ua = ra >> (8 * h), ub = rb >> (8 * h);
-        const uint32_t a0 = sub_f16x2(nibbles_lo(ua), z[grp][0].lo);
-        const uint32_t a1 = sixteenth_minus(nibbles_hi(ua), z[grp][0].hi);
-        const uint32_t a2 = sub_f16x2(nibbles_lo(ub), z[grp][1].lo);
-        const uint32_t a3 = sixteenth_minus(nibbles_hi(ub), z[grp][1].hi);
+        const uint32_t a0 = kv4_value_pair(ra >> (8 * h), z[grp][0]);
+        const uint32_t a1 = kv4_value_pair(ra >> (8 * h + 4), z[grp][0]);
+        const uint32_t a2 = kv4_value_pair(rb >> (8 * h), z[grp][1]);
+        const uint32_t a3 = kv4_value_pair(rb >> (8 * h + 4), z[grp][1]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_f16(st.o[2 * k + h][nt], a0, a1, a2, a3, w[grp][nt][0], w[grp][nt][1]);
-          if constexpr (kTwo)
-            mma_f16(st.o[2 * k + h][nt], a0, a1, a2, a3, rest[grp][nt][0], rest[grp][nt][1]);
+          mma_bf16(st.o[2 * k + h][nt], a0, a1, a2, a3, w[grp][nt][0], w[grp][nt][1]);
+          mma_bf16(st.o[2 * k + h][nt], a0, a1, a2, a3, rest[grp][nt][0], rest[grp][nt][1]);
         }
       }
     }
   }
 }
 
-// Channels `at` + 32 k .. + 3 of a finished row, and with channel 0 its log-sum-exp. A row past its
+// Channels `at` + 32 k .. + 3 (in units of kKv4Unit) of a finished row, and with channel 0 its log-sum-exp. A row past its
 // sequence's count is left alone or filled; what was summed for it means nothing.
 template <typename T, int K>
 __device__ __forceinline__ void kv4_write_row(const Kv4AttnParams& p, int b, int h, int c, int r,
@@ -717,7 +713,7 @@ __device__ __forceinline__ void kv4_write_row(const Kv4AttnParams& p, int b, int
   const Kv4Row row = kv4_row(p, h, c, r);
   const int fill = row.i < p.tokens ? p.fill : 0;
   if (row.live || (fill & LLMFA_KV4_FILL_OUT) != 0) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : 1.f / kKv4Unit / l;
     T* o = static_cast<T*>(p.o.ptr) + b * p.o.sb + row.i * p.o.st + row.hq * p.o.sh + at;
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -806,7 +802,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
     const int n = plan.held[seg.b], c = plan.news[seg.b];
     if (!kEarly) fetch();
     q.template set<T>(p, h, r0, n, c, raw);
-    Kv4State<NT, NG> st;
+    Kv4State<NT> st;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -819,8 +815,6 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
         st.l[nt][k] = 0.f;
       }
     }
-#pragma unroll
-    for (int grp = 0; grp < NG; ++grp) st.top[grp] = 127 - 100;
 
     const int rows = p.tokens * p.group;
     float* scores = p.scores == nullptr ? nullptr
@@ -831,9 +825,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
       ring.wait(p.timeout_ns);
       const int slot0 = t * kKv4TileTokens;
       if (slot0 + kKv4TileTokens > q.all || blocks != 3u)
-        kv4_tile<T, NT, NG, true>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
+        kv4_tile<NT, NG, true>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
       else
-        kv4_tile<T, NT, NG, false>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
+        kv4_tile<NT, NG, false>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
       ring.release();
       loader.template issue<NG>(p, plan, ring, p.row_tiles);
     }
@@ -855,11 +849,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
         const int r = 8 * nt + 2 * cc + j;
         float4 f[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float back = __int_as_float((st.top[k * NG / 4] + 1 - kKv4WeightBits) << 23);  // w's factor
-          f[k] = make_float4(st.o[2 * k][nt][j] * back, st.o[2 * k][nt][2 + j] * back,
-                             st.o[2 * k + 1][nt][j] * back, st.o[2 * k + 1][nt][2 + j] * back);
-        }
+        for (int k = 0; k < 4; ++k)
+          f[k] = make_float4(st.o[2 * k][nt][j], st.o[2 * k][nt][2 + j], st.o[2 * k + 1][nt][j],
+                             st.o[2 * k + 1][nt][2 + j]);
         if (whole) {
           kv4_write_row<T, 4>(p, seg.b, h, c, r0 + r, 4 * g, f, st.m[nt][j], l);
         } else {
