@@ -4,7 +4,7 @@
 // A warp takes 32 tokens at a time:
 //
 //   S^T[token, row] = (K - zero) q^T   mma m16n8k16, A = key codes, B = queries
-//   x = S * scale * row factor         (log2 units, a sum over the groups)
+//   x = S * row factor * scale         (log2 units, a sum over the groups)
 //   p = 2^(x - m), m the row's running maximum
 //   O^T[channel, row] += (V - zero)^T w,   A = value codes, w = p * value scale
 //
@@ -206,7 +206,9 @@ __device__ __forceinline__ Kv4Row kv4_row(const Kv4AttnParams& p, int h, int c, 
 // The query rows of a segment, as a lane's B fragments: of n-tile nt, lane (g,
 // c) has of row g the channels 32 j + 8 c .. + 7, the codes of its word j. Step
 // 2j takes nibbles 0, 4 and 1, 5, step 2j + 1 nibbles 2, 6 and 3, 7. Of rows
-// 2c, 2c + 1, whose scores the lane gets, it has the factor.
+// 2c, 2c + 1, whose scores the lane gets, it has the factor, which is taken in before the key
+// scales: a product of large keys and small queries stays inside fp32. A factor above 1 or below
+// 2^-96 is split into `factor` and one that is taken in afterwards (in shared memory).
 template <int NT>
 struct Kv4Queries {
   static constexpr bool kInRegisters = NT <= 2;  // else in the warp's shared memory
@@ -215,6 +217,7 @@ struct Kv4Queries {
   float factor[NT][2];
   uint32_t limits;  // shared address: slots that each row sees; only tiles at a border read them
   int all;          // slots that every live row sees
+  bool split;       // some row's factor is split; the second parts are behind the limits
 
   __device__ __forceinline__ uint2 operator()(int step, int nt) const {
     if constexpr (kInRegisters) return frag[step][nt];
@@ -247,6 +250,7 @@ struct Kv4Queries {
       const Kv4Row row = kv4_row(p, h, c, r0 + r);
       st_shared_u32(limits + 4 * r, row.live ? kv4_visible(n, c, row.i, p.causal) : 0);
     }
+    bool any_after = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float x[4][8], top = 0.f, bad = 0.f;
@@ -285,12 +289,26 @@ struct Kv4Queries {
           shared[((2 * j + 1) * NT + nt) * 32 + lane] = make_uint2(y[2], y[3]);
         }
       }
-      const float f = bad == 0.f ? ldexpf(p.scale_log2, -e) : __int_as_float(0x7fc00000);
+      float f = ldexpf(p.scale_log2, -e), after = 1.f;
+      if (f > 0x1p96f) {
+        after = ldexpf(p.scale_log2, -e - 32);
+        f = 0x1p32f;
+      } else if (f > 1.f) {
+        after = f;
+        f = 1.f;
+      } else if (f < 0x1p-96f) {
+        after = 0x1p-64f;
+        f = ldexpf(p.scale_log2, 64 - e);
+      }
+      if (bad != 0.f) f = __int_as_float(0x7fc00000);
+      any_after |= after != 1.f;
+      if (cc == 0) st_shared_u32(limits + 4 * (8 * NT + 8 * nt + (lane >> 2)), __float_as_uint(after));
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         factor[nt][k] = __shfl_sync(0xffffffffu, f, (2 * cc + k) * 4);
       }
     }
+    split = __any_sync(0xffffffffu, any_after);
     all = p.causal ? kv4_visible(n, c, r0 / p.group, true) : n;
     __syncwarp();
   }
@@ -298,6 +316,10 @@ struct Kv4Queries {
   __device__ __forceinline__ int2 limit(int nt) const {
     const uint2 v = ld_shared_v2(limits + (8 * nt + 2 * (threadIdx.x & 3)) * 4);
     return make_int2(v.x, v.y);
+  }
+  __device__ __forceinline__ float2 after(int nt) const {
+    const uint2 v = ld_shared_v2(limits + (8 * NT + 8 * nt + 2 * (threadIdx.x & 3)) * 4);
+    return make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
   }
 };
 
@@ -480,7 +502,7 @@ __device__ __forceinline__ void kv4_make_plan(const Kv4AttnParams& p, int hr, ui
 __device__ __forceinline__ int kv4_worker() { return (threadIdx.x >> 5) * gridDim.x + blockIdx.x; }
 
 // Key codes of 16 tokens times the query rows: x of tokens a (row g of the
-// instruction) and a + 8, in log2 units but for the row factor.
+// instruction) and a + 8, in log2 units.
 template <int NT, int NG>
 __device__ __forceinline__ void kv4_scores(uint32_t block, int tok, const Kv4Queries<NT>& q,
                                            float (&x)[NT][4]) {
@@ -519,9 +541,17 @@ __device__ __forceinline__ void kv4_scores(uint32_t block, int tok, const Kv4Que
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float sc = k < 2 ? sa : sb;
-        x[nt][k] = grp == 0 ? raw[nt][k] * sc : fmaf(raw[nt][k], sc, x[nt][k]);
+        const float sc = k < 2 ? sa : sb, y = raw[nt][k] * q.factor[nt][k & 1];
+        x[nt][k] = grp == 0 ? y * sc : fmaf(y, sc, x[nt][k]);
       }
+  }
+  if (q.split) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float2 f = q.after(nt);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[nt][k] *= (k & 1) == 0 ? f.x : f.y;
+    }
   }
 }
 
@@ -552,10 +582,6 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT>& st, uint32_t tile, int to
     for (int u = 0; u < 2; ++u)
       ld_pairs<NG>(block + kv4_half_bytes(NG) + kKv4Block * kKv4RowBytes + (tok + 8 * u) * 4 * NG,
                    pv[s][u]);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[s][nt][k] *= q.factor[nt][k & 1];
     if constexpr (RAGGED) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -751,7 +777,7 @@ struct Kv4AttnSmem {
   Kv4Plan plan;
   Kv4Segment seg[WARPS];
   uint64_t bar[WARPS][STAGES + 1];  // and the ring's flags
-  uint2 limit[WARPS][4 * NT];
+  uint2 limit[WARPS][2 * 4 * NT];   // and second factors
 };
 
 template <typename T, int NT, int NG, int WARPS, int STAGES, int CTAS>
@@ -962,7 +988,7 @@ struct Kv4WeightsSmem {
   Kv4Plan plan;
   Kv4Segment seg[WARPS];
   uint64_t bar[WARPS][STAGES + 1];  // and the ring's flags
-  uint2 limit[WARPS][4 * NT];
+  uint2 limit[WARPS][2 * 4 * NT];   // and second factors
 };
 
 template <typename T, int NT, int NG, int WARPS, int STAGES, int CTAS>
@@ -1033,7 +1059,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
               const int2 limit = q.limit(nt);
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                const float pr = ptx::ex2_mufu(fmaf(x[nt][2 * u + k], q.factor[nt][k], -lse[nt][k]));
+                const float pr = ptx::ex2_mufu(x[nt][2 * u + k] - lse[nt][k]);
                 w += slot < (k == 0 ? limit.x : limit.y) ? pr : 0.f;
               }
             }

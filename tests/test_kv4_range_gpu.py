@@ -62,8 +62,9 @@ def hold(k, v, lens, page=64, group=64, dtype=torch.bfloat16):
 
 def check(got, q, cache, table, lens, *, chain=None, causal=True, scale=1 / math.sqrt(128),
           rows=slice(None)):
-    """Compares o and lse of new tokens `rows` (all sequences have all of q's) and returns the fp64
-    weights. chain: tokens that one worker sums, at most (default: all)."""
+    """Compares o and lse of new tokens `rows` (all sequences have all of q's) and returns the
+    fp64 weights that each token received and what errors of scores move them by, to first order.
+    chain: tokens that one worker sums, at most (default: all)."""
     pages, tab = cache.pages.cpu().numpy(), table.cpu().numpy()
     B, T, Hq, _ = q.shape
     G = Hq // cache.heads
@@ -95,7 +96,8 @@ def check(got, q, cache, table, lens, *, chain=None, causal=True, scale=1 / math
         ltol = (w * dx).sum(-1).permute(0, 2, 1).flatten(0, 1)
         ltol = ltol + (c / 4 + 64) * 2.0 ** -23 + 2.0 ** -21 + 2.0 ** -22 * lse.abs()
         assert bool(((lse_got[b] - lse).abs() <= ltol).all()), b
-        sums.append(w.sum((1, 2)))
+        off = w * (dx + (w * dx).sum(-1, keepdim=True))
+        sums.append((w.sum((1, 2)), off.sum((1, 2))))
     assert device_status() == 0
     return sums
 
@@ -196,6 +198,44 @@ def test_values_near_the_ends_of_the_type(size):
     q = q.to(torch.bfloat16).cuda()
     got = kv4_attention(q, cache, table, ints([n, 1]), return_lse=True)
     check(got, q, cache, table, [n, 1])
+
+
+@pytest.mark.parametrize("query,key", [
+    (-105, 106), (-124, 123), (-130, 122), (-60, 60), (100, -101), (124, -114),
+])
+@pytest.mark.parametrize("decay", [None, 0.0])
+def test_scores_of_ordinary_size_from_queries_and_keys_of_any(query, key, decay):
+    """Powers of two whose product is ordinary, beside a row whose queries are ordinary and, for
+    small keys, sees only scores near 0."""
+    B, H, n, G = 2, 2, 300, 4
+    q, k, v = normal(B, 1, G * H, 128, seed=1), normal(B, n, H, 128, seed=2), normal(B, n, H, 128, seed=3)
+    q = q.clamp(-3.5, 3.5) * 2.0 ** query
+    k = k.clamp(-3.5, 3.5) * 2.0 ** key
+    if key < 0:
+        q[:, :, 1] *= 2.0 ** -query
+    for group in (32, 128):
+        cache, table = hold(k, v, [n] * B, group=group)
+        qc = q.to(torch.bfloat16).cuda()
+        got = kv4_attention(qc, cache, table, ints([n] * B), return_lse=True, decay=decay)
+        sums = check(got, qc, cache, table, [n] * B)
+        if decay is not None:
+            # e^x - 1 <= 2 x up to 1.25, which errors of scores below 2^13 (dx < 0.2) stay under; then
+            # G + 3 fp32 roundings and the sums' (n / 4 + 64) * 2^-23
+            i = torch.arange(n, device="cuda")
+            for b, (want, off) in enumerate(sums):
+                w = cache.weights[table[b, i // 64].long(), :, i % 64].double().T
+                tol = 2 * off + ((G + 3) * 2.0 ** -24 + (n / 4 + 64) * 2.0 ** -23) * want + 1e-30
+                assert bool(((w - want).abs() <= tol).all())
+
+
+def test_a_softmax_scale_far_from_one():
+    B, H, n = 2, 2, 300
+    q, k, v = normal(B, 1, 2 * H, 128, seed=1), normal(B, n, H, 128, seed=2), normal(B, n, H, 128, seed=3)
+    for power, scale in ((100, 2.0 ** -103), (-100, 2.0 ** 97), (-20, 2.0 ** 17), (110, 2.0 ** -113)):
+        cache, table = hold(k, v, [n] * B)
+        qc = (q * 2.0 ** power).to(torch.bfloat16).cuda()
+        got = kv4_attention(qc, cache, table, ints([n] * B), return_lse=True, softmax_scale=scale)
+        check(got, qc, cache, table, [n] * B, scale=scale)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
