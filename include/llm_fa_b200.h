@@ -294,7 +294,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
                         float decay, int fill, int dtype, void* workspace, uint64_t workspace_bytes,
                         void* stream);
 
-/* Workspace of llmfa_kv4_evict_select, 16-byte aligned. */
+/* Workspace of llmfa_kv4_evict_select, 16-byte aligned; keep is at most 2^31 - 8192. */
 int llmfa_kv4_evict_workspace_size(int64_t batch, int64_t heads, int64_t keep, uint64_t* bytes);
 
 /*

@@ -417,7 +417,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
 
 int llmfa_kv4_evict_workspace_size(int64_t batch, int64_t heads, int64_t keep, uint64_t* bytes) {
   if (bytes == nullptr || batch < 1 || heads < 1 || keep < 1) return LLMFA_ERR_INVALID_ARGUMENT;
-  if (batch > kKv4MaxBatch || heads > 1024 || keep >= (int64_t(1) << 31)) return LLMFA_ERR_UNSUPPORTED;
+  if (batch > kKv4MaxBatch || heads > 1024 || keep > kKv4SelectMaxKeep) return LLMFA_ERR_UNSUPPORTED;
   *bytes = static_cast<uint64_t>(batch * heads * keep) * 4;
   return LLMFA_OK;
 }

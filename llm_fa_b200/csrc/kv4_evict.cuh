@@ -77,6 +77,8 @@ constexpr int kKv4SelectMaxWarps = 32;
 constexpr int kKv4SelectMaxCluster = 8;
 constexpr int kKv4SelectKeys = 49152;  // keys that fit a CTA's shared memory (192 KB)
 constexpr int kKv4SelectBins = 256;
+// A cluster's threads walk src in steps of their number, in 32 bits.
+constexpr long long kKv4SelectMaxKeep = (1ll << 31) - kKv4SelectMaxCluster * kKv4SelectMaxWarps * 32;
 
 // Slots of a row for each of a CTA's warps.
 __host__ __device__ constexpr int kv4_select_row(int warps) { return 4 * 32 * warps; }

@@ -298,9 +298,9 @@ def kv4_evict_select(cache: KV4Cache, page_table: torch.Tensor, lengths: torch.T
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise RuntimeError(f"keep must be at least 1 and recent 0 to keep, got {keep}, {recent}")
+    nbytes = _size("llmfa_kv4_evict_workspace_size", B, cache._heads, keep)
     src = torch.empty(B, cache._heads, keep, dtype=torch.int32, device=cache._device)
     new = torch.empty(B, dtype=torch.int32, device=cache._device)
-    nbytes = _size("llmfa_kv4_evict_workspace_size", B, cache._heads, keep)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=cache._device)
     _call(cache, "llmfa_kv4_evict_select", seqs,
           None if seen is None else _ints(seen, "seen", cache, B), keep, recent, src.data_ptr(),

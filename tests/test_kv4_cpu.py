@@ -188,6 +188,14 @@ def test_select_refuses_without_cuda(L, kw, code):
     assert _select(L, **kw) == code
 
 
+@pytest.mark.parametrize("keep", [2 ** 31 - 1, 2 ** 31 - 8191])
+def test_select_refuses_a_budget_whose_last_step_passes_32_bits(L, keep):
+    assert _select(L, keep=keep, ws_bytes=1 << 60) == UNSUP
+    n = ctypes.c_uint64(0)
+    assert L.llmfa_kv4_evict_workspace_size(1, 1, keep, ctypes.byref(n)) == UNSUP
+    assert L.llmfa_kv4_evict_workspace_size(1, 1, 2 ** 31 - 8192, ctypes.byref(n)) == _lib.LLMFA_OK
+
+
 @pytest.mark.parametrize("kw,code", SHARED + [
     (dict(src=0), BAD), (dict(keep=0), BAD), (dict(src=18), UNSUP), (dict(keep=1 << 31), UNSUP)])
 def test_move_refuses_without_cuda(L, kw, code):
