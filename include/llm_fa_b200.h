@@ -257,8 +257,8 @@ int llmfa_kv4_append(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, c
 
 /*
  * Reads slots lengths[b] .. lengths[b] + counts[b] - 1 back into k, v [batch,
- * tokens, heads, 128]; rows past a count are zeros. (seqs->lengths is the
- * first slot to read here.)
+ * tokens, heads, 128], which may share no element; rows past a count are
+ * zeros. (seqs->lengths is the first slot to read here.)
  */
 int llmfa_kv4_expand(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, void* k,
                      const int64_t k_strides[3], void* v, const int64_t v_strides[3],
@@ -278,8 +278,8 @@ int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t hea
  * o = softmax(q k^T * softmax_scale) v for the last counts[b] tokens of each
  * sequence (counts = NULL: all `tokens`); q, o are [batch, tokens, heads_q,
  * 128], heads_q a multiple of the cache's heads, query head i reading key head
- * i / (heads_q / heads); o may not alias q. seqs->lengths counts the new tokens, whose keys are
- * appended already. With causal != 0, new token i sees slots 0 .. lengths[b] -
+ * i / (heads_q / heads); o may share no element with q, nor its rows with one another
+ * (LLMFA_ERR_INVALID_ARGUMENT). seqs->lengths counts the new tokens, whose keys are appended already. With causal != 0, new token i sees slots 0 .. lengths[b] -
  * counts[b] + i, else all. A row that sees no slot gets zeros (and lse -inf);
  * rows past a count get what `fill` says. lse as for llmfa_forward_lse, or
  * NULL. decay >= 0 (at most 1) tracks: weights[slot] = decay * weights[slot] +
@@ -305,7 +305,7 @@ int llmfa_kv4_evict_workspace_size(int64_t batch, int64_t heads, int64_t keep, u
  * recent), go after all others. The freed slots below keep take, in ascending
  * order, the surviving tokens at or above it: src[b][head][d] is the slot
  * whose token slot d is to hold, -1 past the new length min(lengths[b], keep),
- * which new_lengths[b] receives (it must not be seqs->lengths itself). Tables
+ * which new_lengths[b] receives (it may not overlap seqs->lengths). Tables
  * of more than about 14 million slots are LLMFA_ERR_UNSUPPORTED.
  */
 int llmfa_kv4_evict_select(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs,

@@ -12,6 +12,7 @@
 #include "kv4_attention.cuh"
 #include "kv4_evict.cuh"
 #include "kv4_quant.cuh"
+#include "kv4_views.h"
 #include "setup.h"
 
 namespace {
@@ -61,6 +62,19 @@ int check_rows(const void* ptr, const int64_t* st, int64_t batch, int64_t tokens
   }
   *view = Kv4RowView{const_cast<void*>(ptr), use[0], use[1], use[2]};
   return LLMFA_OK;
+}
+
+// What a kernel writes through `a` neither meets itself nor what it reads or writes through `b`,
+// two views of the same shape.
+int check_apart(const Kv4RowView& a, const Kv4RowView& b, int64_t batch, int64_t tokens,
+                int64_t heads) {
+  const auto view = [&](const Kv4RowView& v) {
+    return Kv4View{reinterpret_cast<uintptr_t>(v.ptr), {v.sb, v.st, v.sh}, {batch, tokens, heads}};
+  };
+  const Kv4View out = view(a), other = view(b);
+  return Kv4Meeting(out, nullptr).found() || Kv4Meeting(out, &other).found()
+             ? LLMFA_ERR_INVALID_ARGUMENT
+             : LLMFA_OK;
 }
 
 int check_tokens(int64_t tokens, int dtype, const int32_t* counts) {
@@ -330,6 +344,9 @@ int llmfa_kv4_expand(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, v
   if ((rc = check_rows(v, v_strides, seqs->batch, tokens, cache->heads, &p.v)) != LLMFA_OK) return rc;
   dim3 grid;
   if ((rc = quant_grid(seqs->batch, tokens, cache->heads, &grid)) != LLMFA_OK) return rc;
+  if ((rc = check_apart(p.k, p.v, seqs->batch, tokens, cache->heads)) != LLMFA_OK ||
+      (rc = check_apart(p.v, p.k, seqs->batch, tokens, cache->heads)) != LLMFA_OK)
+    return rc;
   if ((rc = device_status_ptr(&p.seqs.status)) != LLMFA_OK) return rc;
   p.counts = counts;
   p.tokens = static_cast<int>(tokens);
@@ -384,6 +401,7 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
   if (workspace == nullptr || !aligned(workspace, 16)) return LLMFA_ERR_INVALID_ARGUMENT;
   const AttnLayout ws = attn_layout(shape, decay >= 0.f ? capacity : 0);
   if (workspace_bytes < ws.bytes) return LLMFA_ERR_INVALID_ARGUMENT;
+  if ((rc = check_apart(p.o, p.q, seqs->batch, tokens, heads_q)) != LLMFA_OK) return rc;
   int sms = 0;
   if ((rc = device_status_ptr(&p.seqs.status)) != LLMFA_OK || (rc = device_sms(&sms)) != LLMFA_OK)
     return rc;
@@ -437,6 +455,10 @@ int llmfa_kv4_evict_select(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* s
   if (workspace == nullptr || workspace_bytes < need) return LLMFA_ERR_INVALID_ARGUMENT;
   if (!aligned(seen, 4) || !aligned(src, 4) || !aligned(new_lengths, 4) || !aligned(workspace, 16))
     return LLMFA_ERR_UNSUPPORTED;
+  // one block writes a new length while others read the old one
+  const uintptr_t was = reinterpret_cast<uintptr_t>(seqs->lengths);
+  const uintptr_t is = reinterpret_cast<uintptr_t>(new_lengths), bytes = 4 * seqs->batch;
+  if (was < is + bytes && is < was + bytes) return LLMFA_ERR_INVALID_ARGUMENT;
   if ((rc = device_status_ptr(&p.seqs.status)) != LLMFA_OK) return rc;
   p.seen = seen;
   p.src = src;

@@ -206,7 +206,8 @@ def kv4_expand(cache: KV4Cache, page_table: torch.Tensor, start: torch.Tensor, t
                counts: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
                out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """(k, v) [batch, tokens, heads, 128] of slots start[b] .. start[b] + counts[b] - 1 (counts
-    default: tokens); rows past a count are zeros. With `out`, fills and returns that pair."""
+    default: tokens); rows past a count are zeros. With `out`, fills and returns that pair, which
+    may share no element."""
     seqs = _seqs(cache, page_table, start)
     B = seqs.batch
     if out is None:
@@ -239,6 +240,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
     many of its rows are real: they are the last counts[b] tokens of the sequence. With causal,
     each sees the slots up to its own, otherwise all. A row that sees nothing gives zeros and an
     lse of -inf. Rows past a count are left as they were in `out`; without `out` they are zeros.
+    `out` may share a tensor with q, as another slice of it, but no element.
 
     decay (0 to 1) also tracks the weight that each token received: cache.weights becomes
     decay * cache.weights + the softmax weights of this call, summed over the new tokens and the
