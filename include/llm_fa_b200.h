@@ -285,7 +285,8 @@ int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t hea
  * NULL. decay >= 0 (at most 1) tracks: weights[slot] = decay * weights[slot] +
  * the slot's softmax weights summed over the new tokens and the query heads of
  * its head; with decay 0 the old value is not read. decay < 0 leaves weights
- * alone.
+ * alone, and so does a call in which a wait of the attention ran out (reported
+ * in the device status word).
  */
 int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, const void* q,
                         const int64_t q_strides[3], void* o, const int64_t o_strides[3],

@@ -147,11 +147,12 @@ struct AttnConfig<3> : AttnShapeOnSm<4, 2, 2> {};
 
 int attn_workers(int nt, int sms) {
   constexpr int per_sm[] = {AttnConfig<1>::kWorkers, AttnConfig<2>::kWorkers, AttnConfig<3>::kWorkers};
+  static_assert(per_sm[0] % 4 == 0 && per_sm[1] % 4 == 0 && per_sm[2] % 4 == 0, "flags read as words");
   return sms * per_sm[nt - 1];
 }
 
 struct AttnLayout {  // byte offsets in the workspace; partial outputs come first
-  uint64_t ml, unit, row_lse, scores, bytes;
+  uint64_t ml, unit, gave_up, row_lse, scores, bytes;
 };
 
 // Tracking keeps the scores up to this size; past it the keys are read again. Kept, 16 sequences of
@@ -164,11 +165,12 @@ constexpr int kMaxSms = 160;
 
 // `capacity`: slots of a sequence where the call tracks, else 0.
 AttnLayout attn_layout(const AttnShape& s, int64_t capacity) {
-  const uint64_t rows = uint64_t(2) * attn_workers(s.nt, kMaxSms) * 8 * s.nt;
+  const uint64_t workers = attn_workers(s.nt, kMaxSms), rows = 2 * workers * 8 * s.nt;
   AttnLayout w;
   w.ml = rows * kKv4Dim * sizeof(float);
   w.unit = w.ml + rows * sizeof(float2);
-  w.row_lse = w.unit + static_cast<uint64_t>(s.units) * sizeof(int2);
+  w.gave_up = w.unit + static_cast<uint64_t>(s.units) * sizeof(int2);
+  w.row_lse = w.gave_up + (capacity > 0 ? (workers + 3) / 4 * 4 : 0);
   const uint64_t rows_all = static_cast<uint64_t>(s.batch * s.heads_q * s.tokens);
   w.scores = (w.row_lse + (capacity > 0 ? rows_all * sizeof(float) : 0) + 15) / 16 * 16;
   const bool keep = capacity > 0 && s.tokens * (s.heads_q / s.heads) <= kKv4SumRows &&
@@ -411,6 +413,8 @@ int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs
   p.part_ml = reinterpret_cast<float2*>(base + ws.ml);
   p.unit = reinterpret_cast<int2*>(base + ws.unit);
   p.row_lse = decay >= 0.f ? reinterpret_cast<float*>(base + ws.row_lse) : nullptr;
+  p.gave_up = decay >= 0.f ? base + ws.gave_up : nullptr;
+  p.workers = attn_workers(shape.nt, sms);
   p.scores = ws.bytes > ws.scores ? reinterpret_cast<float*>(base + ws.scores) : nullptr;
   p.lse = lse;
   p.counts = counts;

@@ -69,10 +69,12 @@ struct Kv4AttnParams {
   float2* part_ml;  // [2 * workers][8 NT]: maximum (log2 units) and sum
   int2* unit;       // [units]: first worker of a unit, and how many
   float* row_lse;   // [batch][tokens][heads_q], log2 units; null without tracking
+  uint8_t* gave_up; // [workers]: 1 where a worker's wait ran out; null without tracking
   float* scores;    // [batch][heads][capacity][rows], log2 units; null where they are not kept
   int heads_q, tokens, causal;
   int fill;  // LLMFA_KV4_FILL_*: what rows past a count get
   int group, row_tiles;
+  int workers;  // of the attention kernel, a multiple of 4
   uint64_t page_stride;  // bytes of a page, all heads
   float scale_log2;  // softmax_scale * log2(e)
   float decay;       // weights = decay * weights + sums
@@ -800,7 +802,10 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   const int worker = kv4_worker();
   Kv4Segment seg;
   bool more = seg.first(plan.split, worker);
-  if (!more) return;
+  if (!more) {
+    if (lane == 0 && p.gave_up != nullptr) p.gave_up[worker] = 0;
+    return;
+  }
 
   Kv4Ring<STAGES, kv4_block_bytes(NG)> ring{ptx::smem_u32(sm.ring[warp]),
                                             ptx::smem_u32(sm.bar[warp])};
@@ -892,6 +897,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
     if (kEarly && more) fetch();
   }
   ring.report(p.seqs);
+  if (lane == 0 && p.gave_up != nullptr) p.gave_up[worker] = ring.failed();
 }
 
 // Joins the pieces of the units that were cut: one block a unit and row; a
@@ -945,6 +951,14 @@ __global__ void __launch_bounds__(kKv4CombineWarps * 32)
 // The weight that a cached token received is the sum over the rows of 2^(x -
 // lse), once the rows' log-sum-exp is final. Where the scores were kept (4
 // bytes a token and row), a thread adds up a token's, in the order of the rows.
+// Weights outlast a call and decide evictions: where a wait of the attention ran
+// out, and scores and log-sum-exps mean nothing, they stay as they were.
+__device__ __forceinline__ bool kv4_gave_up(const Kv4AttnParams& p, int thread, int threads) {
+  const uint32_t* flags = reinterpret_cast<const uint32_t*>(p.gave_up);
+  uint32_t any = 0;
+  for (int i = thread; i < p.workers / 4; i += threads) any |= flags[i];
+  return any != 0;  // as far as this thread has looked
+}
 constexpr int kKv4SumThreads = 256;
 constexpr int kKv4SumRows = 8192;  // most rows (their log-sum-exp is in shared memory)
 __global__ void __launch_bounds__(kKv4SumThreads)
@@ -959,7 +973,7 @@ __global__ void __launch_bounds__(kKv4SumThreads)
     lse_of[r] = row.live ? p.row_lse[(static_cast<long long>(b) * p.tokens + row.i) * p.heads_q + row.hq]
                          : INFINITY;
   }
-  __syncthreads();
+  if (__syncthreads_or(kv4_gave_up(p, threadIdx.x, kKv4SumThreads))) return;
   const long long first = bh * kv4_capacity(p.pool, p.seqs);
   for (int slot = blockIdx.y * kKv4SumThreads + threadIdx.x; slot < n;
        slot += gridDim.y * kKv4SumThreads) {
@@ -1024,7 +1038,16 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
   for (int rt = 0; rt < p.row_tiles; ++rt) {
     loader.start(p, plan, ring, first, !ring.failed(), 1);  // no more after a timeout
     for (int s = 0; s < STAGES; ++s) issue();
-    if (rt == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows' log-sum-exp
+    if (rt == 0) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows' log-sum-exp
+      if (__any_sync(0xffffffffu, kv4_gave_up(p, lane, 32))) {
+        while (ring.pending > 0) {  // no copy may outlive the block
+          ring.wait(p.timeout_ns);
+          ring.release();
+        }
+        break;
+      }
+    }
     Kv4Segment seg = first;
     for (bool more = true; more; more = seg.next(plan.split)) {
       const int h = seg.i, r0 = rt * kRows, n = plan.held[seg.b], c = plan.news[seg.b];
