@@ -249,3 +249,47 @@ def test_precision_of_flat_weights(dtype, G, T, group):
     q = q.to(dtype).cuda()
     got = kv4_attention(q, cache, table, ints([n] * B), return_lse=True)
     check(got, q, cache, table, [n] * B)
+
+
+# ---------------------------------------------------------------- large ones
+def weights_of(cache, table, b, n):
+    i = torch.arange(n, device="cuda")
+    p = cache.page_size
+    return cache.weights[table[b, i // p].long(), :, i % p].double()  # [n, heads]
+
+
+@pytest.mark.parametrize("n,H,G,group,dtype", [
+    (131072, 1, 4, 32, torch.bfloat16), (100001, 2, 2, 128, torch.float16), (40000, 1, 20, 64, torch.bfloat16),
+])
+def test_one_long_sequence_in_hundreds_of_pieces(n, H, G, group, dtype):
+    q, k, v = normal(1, 1, G * H, 128, seed=1), normal(1, n, H, 128, seed=2), normal(1, n, H, 128, seed=3)
+    v += 0.5  # so that outputs are not nearly nothing
+    cache, table = hold(k, v, [n], group=group, dtype=dtype)
+    q = q.to(dtype).cuda()
+    got = kv4_attention(q, cache, table, ints([n]), return_lse=True, decay=0.0)
+    # at least 8 workers on each of a GPU's 100 SMs or more
+    chain = 32 * (n * H // 32 // 800 + 2)
+    want, off = check(got, q, cache, table, [n], chain=chain)[0]
+    err = (weights_of(cache, table, 0, n) - want.T).abs()
+    tol = 2 * off + ((G + 3) * 2.0 ** -24 + (chain / 4 + 64) * 2.0 ** -23) * want + 1e-37
+    assert bool((err <= tol.T).all())
+
+
+@pytest.mark.parametrize("B,T,H,G", [(129, 1, 2, 1), (300, 2, 1, 3), (300, 1, 1, 20), (4096, 1, 1, 4)])
+def test_batches_of_more_sequences_than_a_block_has_threads(B, T, H, G):
+    gen = torch.Generator().manual_seed(B)
+    lens = (T + torch.randint(0, 120, (B,), generator=gen)).tolist()
+    n = max(lens)
+    q, k, v = normal(B, T, G * H, 128, seed=1), normal(B, n, H, 128, seed=2), normal(B, n, H, 128, seed=3)
+    cache, table = hold(k, v, lens, page=16)
+    q = q.to(torch.bfloat16).cuda()
+    lens[5] = 0  # what its pages hold is not for use
+    got = kv4_attention(q, cache, table, ints(lens), return_lse=True, decay=0.0)
+    assert bool((got[0][5] == 0).all()) and bool((got[1][5] == -math.inf).all())
+    some = [b for b in (*range(0, B, max(1, B // 60)), *range(B - 4, B)) if b != 5]
+    part = torch.tensor(some, device="cuda")
+    sums = check([t[part] for t in got], q[part], cache, table[part], [lens[b] for b in some])
+    for b, (want, off) in zip(some, sums):
+        err = (weights_of(cache, table, b, lens[b]) - want.T).abs()
+        tol = 2 * off + ((T * G + 3) * 2.0 ** -24 + (lens[b] / 4 + 64) * 2.0 ** -23) * want + 1e-37
+        assert bool((err <= tol.T).all())
