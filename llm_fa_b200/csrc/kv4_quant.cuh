@@ -27,6 +27,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
+
 #include "kv4_layout.cuh"
 
 namespace llmfa {
@@ -108,11 +110,16 @@ struct Kv4Pair {
   uint32_t word;
 };
 // x / 15, correctly rounded: the product with 1/15 and one correction by its exact remainder
-// (Markstein's scheme; compared with the quotient for every mantissa).
-__device__ __forceinline__ float kv4_fifteenth(float x) {
+// (Markstein's scheme; a test compares it with the quotient for every mantissa, as host code).
+__host__ __device__ __forceinline__ float kv4_fifteenth(float x) {
   constexpr float c = 1.f / 15.f;
+#ifdef __CUDA_ARCH__
   const float q = __fmul_rn(x, c);
   return __fmaf_rn(__fmaf_rn(-15.f, q, x), c, q);
+#else
+  const float q = x * c;
+  return std::fma(std::fma(-15.f, q, x), c, q);
+#endif
 }
 __device__ __forceinline__ Kv4Pair kv4_pair(float lo, float hi) {
   Kv4Pair p;
