@@ -292,7 +292,9 @@ struct Kv4Queries {
         }
       }
       float f = ldexpf(p.scale_log2, -e), after = 1.f;
-      if (f > 0x1p96f) {
+      if (top == 0.f) {  // a row of zeros, or none: any factor will do
+        f = 1.f;
+      } else if (f > 0x1p96f) {
         after = ldexpf(p.scale_log2, -e - 32);
         f = 0x1p32f;
       } else if (f > 1.f) {
