@@ -189,15 +189,16 @@ int llmfa_selftest_wait_timeout(uint32_t timeout_us, void* stream);
  * A paged cache that holds keys and values in 4 bits, attention over it, and
  * eviction from it by the attention weight that its tokens received. Head dim
  * 128; no counterpart in the reference. All calls are stream-ordered, allocate
- * nothing and can be captured in a CUDA graph (after one eager call of the same
- * entry point, type, group and head counts on the device).
+ * nothing and can be captured in a CUDA graph, after one eager call of the same
+ * entry point and shape on the device (type, group, batch, heads, tokens, table
+ * width, tracking or not: each of these may choose another kernel).
  *
  * Device data is not readable before the launch, so what it may hold wrong is
  * found by the kernels and reported in the device status word
  * (llmfa_device_status): a page id outside the pool or a token without a page
  * (the token is not written, counts as absent, or reads as zeros), a length or
  * count outside its range (clamped; nothing is appended behind a negative
- * length), a move from outside the sequence (not made).
+ * length), a move from below keep or outside the table (not made).
  */
 #define LLMFA_DEVICE_STATUS_KV4_BAD_PAGE 0x2001
 #define LLMFA_DEVICE_STATUS_KV4_BAD_LENGTH 0x2002
@@ -286,7 +287,8 @@ int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t hea
  * the slot's softmax weights summed over the new tokens and the query heads of
  * its head; with decay 0 the old value is not read. decay < 0 leaves weights
  * alone, and so does a call in which a wait of the attention ran out (reported
- * in the device status word).
+ * in the device status word). Outputs are sums in fp32, in units of 2^-24: what
+ * is below 2^-99 of them is lost.
  */
 int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, const void* q,
                         const int64_t q_strides[3], void* o, const int64_t o_strides[3],

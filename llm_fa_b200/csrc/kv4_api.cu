@@ -106,8 +106,9 @@ int quant_grid(int64_t batch, int64_t tokens, int64_t heads, dim3* grid) {
 }
 
 // Rows of a key head, cut into tiles of 8 nt. A pass over the cache takes about 2, 3 and 4 parts of
-// time for 8, 16 and 24 rows (8 x 8192 tokens, 8 heads: 31, 40 and 51 us), which decides; tiles of
-// 32 rows, at 81 us, spill registers and win nowhere.
+// time for 8, 16 and 24 rows (8 x 8192 tokens, 8 heads: 31, 41 and 52 us), which decides. Tiles of
+// 24 rows have 255 registers and spill up to 196 bytes a thread, with groups of 32; tiles of 32
+// rows, tried when 24 took 46 us, took 81.
 struct AttnShape {
   int64_t batch, heads, heads_q, tokens;
   int nt, row_tiles;
@@ -156,7 +157,7 @@ struct AttnLayout {  // byte offsets in the workspace; partial outputs come firs
 };
 
 // Tracking keeps the scores up to this size; past it the keys are read again. Kept, 16 sequences of
-// 4097 tokens with 32 heads of one row (8 MB) are tracked in 14 us, read again in 50.
+// 4097 tokens with 32 heads of one row (8 MB) are tracked in 15 us, read again in 50.
 constexpr uint64_t kMostScores = uint64_t(256) << 20;
 
 // The grid uses at most this many SMs (a B200 has 148), so that the workspace's size follows from

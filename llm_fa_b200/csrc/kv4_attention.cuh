@@ -15,16 +15,18 @@
 // and so hold a code in a byte, is emulated by two fp16 products in mma.sync.
 //
 // What bounds it is not the memory but the instructions that make operands of
-// codes: of some 740 a tile (8 rows, groups of 64) 280 belong to the values,
-// 220 to the keys, 130 to the copies; 62 % of the issue slots are taken, by 12
-// warps on an SM that wait on one another's fixed latencies. The matrix pipe is
-// a fifth busy and can be left out without a change in time, the ALU half.
+// codes: some 830 a tile (8 rows, groups of 64; 1040 with groups of 32), the
+// values' the most. 60 to 64 % of the issue slots are taken, by 12 warps on an SM
+// that wait on one another's fixed latencies; the ALU pipe is half busy, the
+// matrix pipe a quarter. With 24 rows (1050 a tile) 8 warps take 40 %, and the
+// matrix pipe is 43 % busy.
 // Measured: 32 sequences of 3.3k to 8.2k tokens, 8 heads, 8 rows: 72 us, 3.0
-// TB/s; one of 131,071 tokens, 8 heads, 4 rows, groups of 32: 59 us, 2.8 TB/s;
+// TB/s; one of 131,071 tokens, 8 heads, 4 rows, groups of 32: 60 us, 2.8 TB/s;
 // without any arithmetic the copies alone take 44 and 35 us, of which 12 are
-// launches, the plan and the first loads. 12 warps on an SM have the 168
-// registers that a tile needs; 14 with 144 and 16 with 128 spill (72 and 68 us,
-// groups of 32: 90 and 93), 8 are 10 % slower.
+// launches, the plan and the first loads. 12 warps on an SM have 168 registers:
+// a tile of 8 rows needs a few more (spills of 8, 20 and 140 bytes a thread for
+// groups of 128, 64 and 32). 14 warps with 144 and 16 with 128 spill more (72 and
+// 68 us when 12 took 64), 8 were 10 % slower.
 //
 // Key codes become fp16 integers by one LOP3 and one HFMA2 a pair: a nibble u in
 // bits 0-3 of a half, or'ed with 0x6400, is 1024 + u, in bits 4-7 it is 1024 +
@@ -38,7 +40,7 @@
 // of it). w is the sum of two bf16 numbers, 2^-18 of it off: bf16 has fp32's
 // range, so that a token's value scale, whatever weight the token has, takes
 // nothing from the precision of another's. (One fp16 number with a common
-// exponent for the scales seen, 64 instead of 72 us for the batch below, loses
+// exponent for the scales seen, 64 instead of 72 us for the batch above, loses
 // the values of tokens whose scales are 2^24 below that of a token of no weight.)
 // Sums, maxima and outputs are fp32; outputs are summed in units of 2^-24, so
 // that weights up to 2^kKv4Slack of many tokens do not pass fp32's range.

@@ -1,8 +1,8 @@
 // Eviction from the 4-bit cache by accumulated attention weight.
 //
 // select: of a sequence's n slots, n - keep go from every head. They are the
-// smallest by (protected, weight, slot), where a slot is protected when its
-// position is one of the `recent` latest. Freed slots below `keep` (holes) and
+// smallest by weight, then slot; slots whose position is one of the `recent`
+// latest are protected: they go after all others, by slot alone. Freed slots below `keep` (holes) and
 // surviving slots at or above it (movers) are equally many; the k-th hole takes
 // the k-th mover. src[d] is the slot whose token slot d holds afterwards (d
 // itself where nothing moves), -1 past the new length.

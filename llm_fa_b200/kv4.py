@@ -12,7 +12,8 @@ scale and a zero for every 32, 64 or 128 channels, a quarter to a third of their
 
 Slot i of sequence b is in page page_table[b, i // page_size]; lengths[b] slots hold tokens. Both
 are int32 tensors on the cache's device that the caller keeps: the layers of a model share them,
-so no call changes them. Prompts that need their prefix in 16 bits read it with kv4_expand.
+so no call changes them. A prompt is appended and attended to with all of its tokens in one call,
+causal among them; kv4_expand gives a range of the cache in 16 bits to whatever else needs it.
 
 As with attention_forward, calls only enqueue work on the current stream, and the arithmetic is
 the library's own kernels. What the device tensors may hold wrong (a page outside the pool, a
