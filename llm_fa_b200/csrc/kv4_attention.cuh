@@ -20,28 +20,29 @@
 // that wait on one another's fixed latencies; the ALU pipe is half busy, the
 // matrix pipe a quarter. With 24 rows (1050 a tile) 8 warps take 40 %, and the
 // matrix pipe is 43 % busy.
-// Measured: 32 sequences of 3.3k to 8.2k tokens, 8 heads, 8 rows: 72 us, 3.0
-// TB/s; one of 131,071 tokens, 8 heads, 4 rows, groups of 32: 60 us, 2.8 TB/s;
+// Measured: 32 sequences of 3.3k to 8.2k tokens, 8 heads, 8 rows: 74 us, 2.9
+// TB/s; one of 131,071 tokens, 8 heads, 4 rows, groups of 32: 61 us, 2.7 TB/s;
 // without any arithmetic the copies alone take 44 and 35 us, of which 12 are
 // launches, the plan and the first loads. 12 warps on an SM have 168 registers:
 // a tile of 8 rows needs a few more (spills of 8, 20 and 140 bytes a thread for
 // groups of 128, 64 and 32). 14 warps with 144 and 16 with 128 spill more (72 and
 // 68 us when 12 took 64), 8 were 10 % slower.
 //
-// Key codes become fp16 integers by one LOP3 and one HFMA2 a pair: a nibble u in
-// bits 0-3 of a half, or'ed with 0x6400, is 1024 + u, in bits 4-7 it is 1024 +
-// 16 u; taking off 1024 + zero (after a multiplication with 1/16 for the
-// latter: 64 + zero) leaves u - zero exactly. Its products with 11-bit numbers
-// are exact in fp32. Value codes become bf16 integers in the same way, by 0x4300
-// (128 + u; the upper nibble is shifted down first, as bf16 has 7 bits).
+// Codes become integers of 16 bits. For fp16 by one LOP3 and one HFMA2 a pair: a
+// nibble u in bits 0-3 of a half, or'ed with 0x6400, is 1024 + u, in bits 4-7 it
+// is 1024 + 16 u; taking off 1024 + zero (after a multiplication with 1/16 for
+// the latter: 64 + zero) leaves u - zero exactly. For bf16 in the same way by
+// 0x4300, 128 + u; the upper nibble is shifted down first, as bf16 has 7 bits.
 //
-// Roundings to 16 bits: q is scaled by a power of two per row so that its
-// largest element is near 2^13 (bf16 and fp16 values stay exact down to 2^-37
-// of it). w is the sum of two bf16 numbers, 2^-18 of it off: bf16 has fp32's
-// range, so that a token's value scale, whatever weight the token has, takes
-// nothing from the precision of another's. (One fp16 number with a common
-// exponent for the scales seen, 64 instead of 72 us for the batch above, loses
-// the values of tokens whose scales are 2^24 below that of a token of no weight.)
+// Roundings to 16 bits: none of queries and keys, whose products are exact in
+// fp32; both have the queries' type. (bf16 queries made fp16 by a power of two a
+// row, 72 instead of 74 us for the batch above, lose channels 2^30 below the
+// row's largest, which count where their keys are as much larger.) w is the sum
+// of two bf16 numbers, 2^-18 of it off: bf16 has fp32's range, so that a token's
+// value scale, whatever weight the token has, takes nothing from the precision of
+// another's. (One fp16 number with a common exponent for the scales seen, 64
+// instead of 72 us, loses the values of tokens whose scales are 2^24 below that
+// of a token of no weight.)
 // Sums, maxima and outputs are fp32; outputs are summed in units of 2^-24, so
 // that weights up to 2^kKv4Slack of many tokens do not pass fp32's range.
 //
@@ -53,6 +54,8 @@
 // and values with their pairs) that a lane issues and the warp waits for, and
 // writes what it has of a unit. Warps of a block share nothing but the plan.
 #pragma once
+#include <type_traits>
+
 #include "../../include/llm_fa_b200.h"
 #include "kv4_plan.cuh"
 #include "kv4_quant.cuh"
@@ -91,21 +94,21 @@ constexpr int kSiteKv4Tile = 13;
 constexpr unsigned long long kKv4DrainNs = 1000000;  // for copies in flight after that
 
 // ---------------------------------------------------------------- instructions
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                        uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+template <typename T>
+__device__ __forceinline__ void mma_16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                       uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Transpose of an 8x8 matrix of 16-bit elements held one row a lane quad.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -184,16 +187,36 @@ __device__ __forceinline__ Kv4Zero kv4_zero(uint32_t pair_a, uint32_t pair_b) {
 }
 // Two codes less their zeros as bf16: 0x4300 + u is 128 + u, whose low nibble alone lies inside the
 // mantissa, and so for the zero, 128 + zero.
-__device__ __forceinline__ uint32_t kv4_value_pair(uint32_t w, uint32_t zero) {
+__device__ __forceinline__ uint32_t kv4_bf16_pair(uint32_t w, uint32_t zero) {
   uint32_t r, d;
   asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(r) : "r"(w));
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(r), "r"(zero));
   return d;
 }
-__device__ __forceinline__ uint32_t kv4_value_zero(uint32_t pair_a, uint32_t pair_b) {
+__device__ __forceinline__ uint32_t kv4_bf16_zero(uint32_t pair_a, uint32_t pair_b) {
   return __byte_perm(__float_as_uint(__uint_as_float(pair_a) + 8405760.f),
                      __float_as_uint(__uint_as_float(pair_b) + 8405760.f), 0x5410);
 }
+// A token's key codes of a group as operands of the queries' type.
+template <typename T>
+struct Kv4Keys {  // bf16
+  uint32_t zero;
+  __device__ __forceinline__ explicit Kv4Keys(uint32_t pair) : zero(kv4_bf16_zero(pair, pair)) {}
+  // Nibbles 0, 4 and 1, 5 of a word, or in the second half 2, 6 and 3, 7.
+  __device__ __forceinline__ void pairs(uint32_t w, int half, uint32_t& first, uint32_t& second) const {
+    first = kv4_bf16_pair(w >> (8 * half), zero);
+    second = kv4_bf16_pair(w >> (8 * half + 4), zero);
+  }
+};
+template <>
+struct Kv4Keys<__half> {
+  Kv4Zero zero;
+  __device__ __forceinline__ explicit Kv4Keys(uint32_t pair) : zero(kv4_zero(pair, pair)) {}
+  __device__ __forceinline__ void pairs(uint32_t w, int half, uint32_t& first, uint32_t& second) const {
+    first = sub_f16x2(nibbles_lo(w >> (8 * half)), zero.lo);
+    second = sixteenth_minus(nibbles_hi(w >> (8 * half)), zero.hi);
+  }
+};
 __device__ __forceinline__ float kv4_scale(uint32_t pair) { return __uint_as_float(pair << 16); }
 
 // ---------------------------------------------------------------- query rows
@@ -275,16 +298,18 @@ struct Kv4Queries {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         bad += __shfl_xor_sync(0xffffffffu, bad, d);
       }
-      // 2^e brings the row's largest element to [2^13, 2^14). A row with an infinity or a NaN is
-      // zeros with a NaN factor: it becomes NaN, the others do not.
-      const int e = min(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 126);
+      // 2^e keeps sums of products with codes inside fp32 (128 of up to 15 times the largest element),
+      // and rows of the smallest numbers in its normal range; fp16 needs neither. A row with an
+      // infinity or a NaN is zeros with a NaN factor: it becomes NaN, the others do not.
+      const int t = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+      const int e = std::is_same<T, __half>::value ? 0 : t > 115 ? 115 - t : t < -60 ? -60 - t : 0;
       const float up = __int_as_float((e + 127) << 23);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t y[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          y[k] = bad == 0.f ? Kv4Type<__half>::pack(x[j][k] * up, x[j][k + 4] * up) : 0u;
+          y[k] = bad == 0.f ? Kv4Type<T>::pack(x[j][k] * up, x[j][k + 4] * up) : 0u;
         if constexpr (kInRegisters) {
           frag[2 * j][nt] = make_uint2(y[0], y[1]);
           frag[2 * j + 1][nt] = make_uint2(y[2], y[3]);
@@ -509,7 +534,7 @@ __device__ __forceinline__ int kv4_worker() { return (threadIdx.x >> 5) * gridDi
 
 // Key codes of 16 tokens times the query rows: x of tokens a (row g of the
 // instruction) and a + 8, in log2 units.
-template <int NT, int NG>
+template <typename T, int NT, int NG>
 __device__ __forceinline__ void kv4_scores(uint32_t block, int tok, const Kv4Queries<NT>& q,
                                            float (&x)[NT][4]) {
   const uint32_t row = block + tok * kKv4RowBytes + (threadIdx.x & 3) * 16;
@@ -521,7 +546,7 @@ __device__ __forceinline__ void kv4_scores(uint32_t block, int tok, const Kv4Que
   const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
   for (int grp = 0; grp < NG; ++grp) {
-    const Kv4Zero za = kv4_zero(pa[grp], pa[grp]), zb = kv4_zero(pb[grp], pb[grp]);
+    Kv4Keys<T> ka(pa[grp]), kb(pb[grp]);
     float raw[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -531,14 +556,13 @@ __device__ __forceinline__ void kv4_scores(uint32_t block, int tok, const Kv4Que
     for (int j = grp * 4 / NG; j < (grp + 1) * 4 / NG; ++j) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const uint32_t ua = wa[j] >> (8 * half), ub = wb[j] >> (8 * half);
-        const uint32_t a0 = sub_f16x2(nibbles_lo(ua), za.lo), a1 = sub_f16x2(nibbles_lo(ub), zb.lo);
-        const uint32_t a2 = sixteenth_minus(nibbles_hi(ua), za.hi);
-        const uint32_t a3 = sixteenth_minus(nibbles_hi(ub), zb.hi);
+        uint32_t a0, a1, a2, a3;
+        ka.pairs(wa[j], half, a0, a2);
+        kb.pairs(wb[j], half, a1, a3);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const uint2 f = q(2 * j + half, nt);
-          mma_f16(raw[nt], a0, a1, a2, a3, f.x, f.y);
+          mma_16<T>(raw[nt], a0, a1, a2, a3, f.x, f.y);
         }
       }
     }
@@ -571,7 +595,7 @@ struct Kv4State {
 // One tile of 32 tokens. RAGGED: some row does not see all of it (or a block is
 // missing): `blocks` says which are here, n what the sequence holds. `scores`,
 // if not null, takes the scores of rows r0 .. of the head's `rows`.
-template <int NT, int NG, bool RAGGED>
+template <typename T, int NT, int NG, bool RAGGED>
 __device__ __forceinline__ void kv4_tile(Kv4State<NT>& st, uint32_t tile, int tok,
                                          const Kv4Queries<NT>& q, uint32_t blocks, int slot0, int n,
                                          float* scores, int rows, int r0) {
@@ -583,7 +607,7 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT>& st, uint32_t tile, int to
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const uint32_t block = tile + s * kBlockBytes;
-    kv4_scores<NT, NG>(block, tok, q, x[s]);
+    kv4_scores<T, NT, NG>(block, tok, q, x[s]);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
       ld_pairs<NG>(block + kv4_half_bytes(NG) + kKv4Block * kKv4RowBytes + (tok + 8 * u) * 4 * NG,
@@ -711,8 +735,8 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT>& st, uint32_t tile, int to
       }
 #pragma unroll
       for (int grp = 0; grp < NG; ++grp) {
-        z[grp][0] = kv4_value_zero(pz[0][grp], pz[1][grp]);
-        z[grp][1] = kv4_value_zero(pz[2][grp], pz[3][grp]);
+        z[grp][0] = kv4_bf16_zero(pz[0][grp], pz[1][grp]);
+        z[grp][1] = kv4_bf16_zero(pz[2][grp], pz[3][grp]);
       }
     }
 #pragma unroll
@@ -723,14 +747,14 @@ __device__ __forceinline__ void kv4_tile(Kv4State<NT>& st, uint32_t tile, int to
       const uint32_t rb = k < 2 ? __byte_perm(v[2].x, v[3].x, sel) : __byte_perm(v[2].y, v[3].y, sel);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t a0 = kv4_value_pair(ra >> (8 * h), z[grp][0]);
-        const uint32_t a1 = kv4_value_pair(ra >> (8 * h + 4), z[grp][0]);
-        const uint32_t a2 = kv4_value_pair(rb >> (8 * h), z[grp][1]);
-        const uint32_t a3 = kv4_value_pair(rb >> (8 * h + 4), z[grp][1]);
+        const uint32_t a0 = kv4_bf16_pair(ra >> (8 * h), z[grp][0]);
+        const uint32_t a1 = kv4_bf16_pair(ra >> (8 * h + 4), z[grp][0]);
+        const uint32_t a2 = kv4_bf16_pair(rb >> (8 * h), z[grp][1]);
+        const uint32_t a3 = kv4_bf16_pair(rb >> (8 * h + 4), z[grp][1]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_bf16(st.o[2 * k + h][nt], a0, a1, a2, a3, w[grp][nt][0], w[grp][nt][1]);
-          mma_bf16(st.o[2 * k + h][nt], a0, a1, a2, a3, rest[grp][nt][0], rest[grp][nt][1]);
+          mma_16<__nv_bfloat16>(st.o[2 * k + h][nt], a0, a1, a2, a3, w[grp][nt][0], w[grp][nt][1]);
+          mma_16<__nv_bfloat16>(st.o[2 * k + h][nt], a0, a1, a2, a3, rest[grp][nt][0], rest[grp][nt][1]);
         }
       }
     }
@@ -860,9 +884,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
       ring.wait(p.timeout_ns);
       const int slot0 = t * kKv4TileTokens;
       if (slot0 + kKv4TileTokens > q.all || blocks != 3u)
-        kv4_tile<NT, NG, true>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
+        kv4_tile<T, NT, NG, true>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
       else
-        kv4_tile<NT, NG, false>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
+        kv4_tile<T, NT, NG, false>(st, ring.tile(), tok, q, blocks, slot0, n, scores, rows, r0);
       ring.release();
       loader.template issue<NG>(p, plan, ring, p.row_tiles);
     }
@@ -1076,7 +1100,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           float x[NT][4];
-          kv4_scores<NT, NG>(tile + s * kv4_half_bytes(NG), tok, q, x);
+          kv4_scores<T, NT, NG>(tile + s * kv4_half_bytes(NG), tok, q, x);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int slot = slot0 + 16 * s + tok + 8 * u;

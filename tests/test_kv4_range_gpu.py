@@ -228,6 +228,24 @@ def test_scores_of_ordinary_size_from_queries_and_keys_of_any(query, key, decay)
                 assert bool(((w - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("power", [20, 36, 50, 90])
+@pytest.mark.parametrize("G", [4, 20])
+def test_channels_of_a_query_of_very_different_size(power, G):
+    """Half of the channels are large in queries and as small in keys: both halves count."""
+    B, H, n = 2, 2, 300
+    q, k, v = normal(B, 1, G * H, 128, seed=1), normal(B, n, H, 128, seed=2), normal(B, n, H, 128, seed=3)
+    q[..., :64] *= 2.0 ** power
+    k[..., :64] *= 2.0 ** -power
+    for group in (32, 64):
+        cache, table = hold(k, v, [n] * B, group=group)
+        qc = q.to(torch.bfloat16).cuda()
+        got = kv4_attention(qc, cache, table, ints([n] * B), return_lse=True, decay=0.0)
+        sums = check(got, qc, cache, table, [n] * B)
+        for b, (want, off) in enumerate(sums):
+            tol = 2 * off + ((G + 3) * 2.0 ** -24 + (n / 4 + 64) * 2.0 ** -23) * want + 1e-37
+            assert bool(((weights_of(cache, table, b, n) - want.T).abs() <= tol.T).all())
+
+
 def test_a_softmax_scale_far_from_one():
     B, H, n = 2, 2, 300
     q, k, v = normal(B, 1, 2 * H, 128, seed=1), normal(B, n, H, 128, seed=2), normal(B, n, H, 128, seed=3)
