@@ -4,8 +4,8 @@
 //   scale = bf16((hi - lo) / 15)     zero = clamp(round(-lo / scale), 0, 15)
 //   code  = clamp(round(x / scale) + zero, 0, 15)       (halves to even)
 // The range always takes in 0, so zero is an integer code and 0 is held
-// exactly. A group with an infinity, a NaN or a range past fp32 is stored with
-// a NaN scale: whoever reads it gets NaN, not a wrong number.
+// exactly. A group with an infinity or a NaN is stored with a NaN scale: whoever
+// reads it gets NaN, not a wrong number.
 //
 // The rounding is exact. x has at most 11 significant bits and scale 8, so
 // x / scale is either a half-integer or at least 2^-12 away from one. The
@@ -123,9 +123,10 @@ __host__ __device__ __forceinline__ float kv4_fifteenth(float x) {
 }
 __device__ __forceinline__ Kv4Pair kv4_pair(float lo, float hi) {
   Kv4Pair p;
-  const float span = __fsub_rn(hi, lo);
-  float s = __bfloat162float(__float2bfloat16_rn(kv4_fifteenth(span)));
-  // a NaN or an infinity in the group shows in hi - lo
+  // of halves: hi - lo itself may pass fp32's range
+  const float span = __fmaf_rn(hi, 0.5f, -0.5f * lo);
+  float s = 2.f * __bfloat162float(__float2bfloat16_rn(kv4_fifteenth(span)));
+  // a NaN or an infinity in the group shows in their difference
   if (!(span < __int_as_float(0x7f800000))) s = __int_as_float(0x7fc00000);
   // Below 2^-120 the reciprocal nears the end of fp32's range: such a group counts as zeros.
   if (s < 0x1p-120f) s = 0.f;

@@ -7,8 +7,9 @@
 #include "../../llm_fa_b200/csrc/kv4_quant.cuh"
 
 int main() {
-  // 2^-117 is below the least span whose scale counts, 15 * 2^-120; 2^127 the largest exponent
-  for (int e : {-117, -116, -60, -1, 0, 3, 126, 127}) {
+  // halves of spans: 2^-118 is below that of the least whose scale counts, 15 * 2^-120; 2^127 is the
+  // largest exponent
+  for (int e : {-118, -117, -116, -60, -1, 0, 3, 126, 127}) {
     for (uint32_t m = 0; m < (1u << 23); ++m) {
       const float x = std::ldexp(1.f + std::ldexp(static_cast<float>(m), -23), e);
       const volatile float by = 15.f;

@@ -102,6 +102,26 @@ def check(got, q, cache, table, lens, *, chain=None, causal=True, scale=1 / math
     return sums
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("low", [-3.38e38, -2.0e38, -1.0e36, 0.0])
+def test_append_groups_whose_span_passes_fp32(group, low):
+    """Finite groups are quantised as defined, however wide, and large ones attend."""
+    x = normal(1, 40, 2, 128, seed=int(group)) * 1e37
+    x[:, :, :, ::32], x[:, :, :, 1::32] = 3.38e38, low
+    x = x.to(torch.bfloat16)
+    cache, table = hold(x.double(), -x.double(), [40], group=group)
+    pages, tab = cache.pages.cpu().numpy(), table.cpu().numpy()
+    for h in range(2):
+        for value, y in ((0, x), (1, -x)):
+            want = plain.quantise(y[0, :, h].double().numpy(), group)[0]
+            assert np.array_equal(plain.read(pages, tab[0], 40, 64, group, h, value), want)
+    q = (normal(1, 1, 4, 128, seed=1) * 2.0 ** -124).to(torch.bfloat16).cuda()
+    got = kv4_attention(q, cache, table, ints([40]), return_lse=True)
+    inside = plain.read(pages, tab[0], 40, 64, group, 0, 1)
+    if np.abs(inside).max() < 3.3e38:  # else an output may round to infinity
+        check(got, q, cache, table, [40])
+
+
 # 512 heads of 4 tiles each: a worker has several units, so a segment takes in whole sequences
 MANY = dict(B=64, H=8, n=100)
 
