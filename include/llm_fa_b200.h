@@ -287,7 +287,8 @@ int llmfa_kv4_attention_workspace_size(int64_t batch, int64_t heads, int64_t hea
  * the slot's softmax weights summed over the new tokens and the query heads of
  * its head; with decay 0 the old value is not read. decay < 0 leaves weights
  * alone, and so does a call in which a wait of the attention ran out (reported
- * in the device status word). Outputs are sums in fp32, in units of 2^-24: what
+ * in the device status word); one that ran out in the update itself leaves them
+ * partly updated, and is reported too. Outputs are sums in fp32, in units of 2^-24: what
  * is below 2^-99 of them is lost.
  */
 int llmfa_kv4_attention(const llmfa_kv4_cache* cache, const llmfa_kv4_seqs* seqs, const void* q,

@@ -15,17 +15,17 @@
 // and so hold a code in a byte, is emulated by two fp16 products in mma.sync.
 //
 // What bounds it is not the memory but the instructions that make operands of
-// codes: some 830 a tile (8 rows, groups of 64; 1040 with groups of 32), the
-// values' the most. 60 to 64 % of the issue slots are taken, by 12 warps on an SM
+// codes: some 850 a tile (8 rows, groups of 64; 1050 with groups of 32), the
+// values' the most. 60 to 63 % of the issue slots are taken, by 12 warps on an SM
 // that wait on one another's fixed latencies; the ALU pipe is half busy, the
-// matrix pipe a quarter. With 24 rows (1050 a tile) 8 warps take 40 %, and the
-// matrix pipe is 43 % busy.
+// matrix pipe a quarter. With 24 rows (1050 a tile) 8 warps take 41 %, and the
+// matrix pipe is 44 % busy.
 // Measured: 32 sequences of 3.3k to 8.2k tokens, 8 heads, 8 rows: 74 us, 2.9
 // TB/s; one of 131,071 tokens, 8 heads, 4 rows, groups of 32: 61 us, 2.7 TB/s;
 // without any arithmetic the copies alone take 44 and 35 us, of which 12 are
 // launches, the plan and the first loads. 12 warps on an SM have 168 registers:
-// a tile of 8 rows needs a few more (spills of 8, 20 and 140 bytes a thread for
-// groups of 128, 64 and 32). 14 warps with 144 and 16 with 128 spill more (72 and
+// a tile of 8 rows needs a few more (spills of up to 8, 76 and 140 bytes a thread
+// for groups of 128, 64 and 32). 14 warps with 144 and 16 with 128 spill more (72 and
 // 68 us when 12 took 64), 8 were 10 % slower.
 //
 // Codes become integers of 16 bits. For fp16 by one LOP3 and one HFMA2 a pair: a
